@@ -283,7 +283,7 @@ def _own(s):
             return outs
         return outs + list(torch.autograd.grad(outs, s["leaves"], [s["dy"]] + ([s["ds"]] if case["with_sum"] else [])))
     with torch.set_grad_enabled(case["train"]):
-        y = blocks.embedding(s["table"], s["idx"], weight=s["weight"] if case["weights"] else None, scale=case["scale"])
+        y = blocks.embedding(s["table"], s["idx"], weight=s["weight"] if case["weights"] else None, scale=case["scale"], bag=case["k"] > 1)
     if not case["train"]:
         return [y]
     return [y, *torch.autograd.grad(y, [s["table"]] + ([s["weight"]] if case["weight_grad"] else []), [s["dy"]])]
