@@ -21,8 +21,10 @@ LIB = os.path.join(HERE, "libls3d.so")
 ARCH = "gfx950"
 # -ffp-contract=off: every f32 multiply/add rounds where it is written (voxel centres, distances and the
 # voxel-coordinate division must match the reference bit for bit); fused multiply-adds are explicit fmaf().
+# -packed-fp32-ops: no v_pk_add / mul / fma_f32 (hipcc -O3 forms them from ordinary float code; some of their forms have given wrong
+# results now and then on these cards).  Every f32 operation keeps its value: the packed forms round the same way.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-ffp-contract=off", "-fno-gpu-rdc",
-          "-Wno-unused-result", "-Wno-unused-value"]
+          "-Wno-unused-result", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def sources():
