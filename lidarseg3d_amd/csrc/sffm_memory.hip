@@ -131,6 +131,10 @@ __global__ __launch_bounds__(SM_THREADS) void k_sffm_memory(const float *__restr
   token_phase(0);
   for (int l = 0; l < NL; ++l) {
     const SmLayer &P = prm.layer[l];
+    int tid = threadIdx.x;
+#ifndef HIPSIM
+    asm volatile("" : "+v"(tid));  // as in sm_phase: the phases' addresses are formed where they are used, kept across the layers they spill
+#endif
     __syncthreads();
     SM_MARK()  // 1 + 4 l: q | k | v (+ the previous layer's k / v projections) done
     // ---- softmax(q k^T / sqrt(hd)) v: 16 threads per token = 4 heads x 4 key groups (keys j = g, g + 4, ...); the groups' maxima, sums and
