@@ -779,6 +779,69 @@ int ls3d_layer_norm_forward(const float *x, int n, int c, const float *gamma, co
 int ls3d_layer_norm_backward(const float *x, const float *dy, const float *gamma, const float *stats, int n, int c, float *dx, float *dgamma,
                              float *dbeta, void *workspace, size_t workspace_bytes, ls3d_stream_t stream);
 
+/* ---- training-block operators (lidarseg3d_amd/blocks.py): element types, dropout, residual norm, row lookup ----------------------------------
+ * Rows of any length and alignment; `*_ld` are row strides in elements (>= the row's length); sums, statistics and gradients of parameters are
+ * formed in f32 and rounded to their type once.  Nothing is kept between calls, no atomics: the same inputs give the same bits. */
+#define LS3D_DTYPE_F32 0
+#define LS3D_DTYPE_BF16 1
+#define LS3D_DTYPE_F16 2
+#define LS3D_INDEX_I32 0
+#define LS3D_INDEX_I64 1
+
+/* Dropout with a counter-based mask that is never stored.  Element (row, col) is dropped where its 16-bit draw is below t = round(65536 p), else scaled
+ * by 65536 / (65536 - t) (p is thus resolved to 2^-16 and the expectation is x exactly; p = 1 drops all).  Draws: Philox4x32 with 10 rounds, key = seed,
+ * counter = (col / 8, row, call, step), eight draws a counter, low half words first.  state = (seed, step), two int64 on the DEVICE (read when the kernel runs:
+ * a captured graph draws anew when the step is advanced between replays); call: the call's number within a step.  relu: of relu(x).
+ * A dropped element is 0 whatever x holds there.  backward: the same state, call and p; relu: y is the forward's output (else NULL). */
+int ls3d_dropout_forward(const void *x, long long x_ld, long long rows, long long c, int dtype, float p, const int64_t *state, uint32_t call, int relu,
+                         void *y, ls3d_stream_t stream);
+int ls3d_dropout_backward(const void *dy, long long dy_ld, const void *y, long long rows, long long c, int dtype, float p, const int64_t *state, uint32_t call,
+                          int relu, void *dx, ls3d_stream_t stream);
+
+/* The residual of a transformer block with the norms before and after it, in one pass:
+ *   t = in(x);  s = alpha * residual + gate * dropout(t);  y = out(s)
+ * residual NULL: s = gate * dropout(t); weight NULL reads as 1, bias NULL as 0; gate: one value per channel [c] or per element [n, c] (of x's type).
+ * dtype: x, y, a full gate and their gradients; stream_dtype: residual, s and their gradients - the same type or LS3D_DTYPE_F32.  c <= 8192.
+ *   forward : y (out.kind != NONE) and / or s (either may be NULL, not both), stats[n][4] = mean, 1/std of in, mean, 1/std of out (NULL: not wanted)
+ *   backward: from dy and / or ds (NULL: zero) and the forward's inputs and stats: dx, dresidual, dgate ([c] or [n, c]), dw / db of the norms; a NULL
+ *             output is not formed.  workspace: ls3d_residual_norm_workspace_bytes(n, c) bytes, 16-byte aligned (needed for dw, db and a channel gate). */
+#define LS3D_NORM_NONE 0
+#define LS3D_NORM_LAYER 1
+#define LS3D_NORM_RMS 2
+#define LS3D_GATE_NONE 0
+#define LS3D_GATE_CHANNEL 1
+#define LS3D_GATE_FULL 2
+typedef struct {
+  const void *weight, *bias;
+  int32_t kind, weight_dtype, bias_dtype;
+  float eps;
+} ls3d_norm_t;
+typedef struct {
+  ls3d_norm_t in, out;
+  const void *gate;
+  long long gate_ld;
+  const int64_t *state;
+  int32_t dtype, stream_dtype, gate_kind, gate_dtype;
+  float alpha, p;
+  uint32_t call;
+} ls3d_residual_norm_t;
+int ls3d_residual_norm_forward(const void *x, long long x_ld, const void *residual, long long res_ld, int n, int c, const ls3d_residual_norm_t *desc_host,
+                               void *y, void *sum, float *stats, ls3d_stream_t stream);
+size_t ls3d_residual_norm_workspace_bytes(int n, int c);
+int ls3d_residual_norm_backward(const void *x, long long x_ld, const void *residual, long long res_ld, int n, int c, const ls3d_residual_norm_t *desc_host,
+                                const float *stats, const void *dy, long long dy_ld, const void *ds, long long ds_ld, void *dx, void *dresidual, void *dgate,
+                                void *dw_in, void *db_in, void *dw_out, void *db_out, void *workspace, size_t workspace_bytes, ls3d_stream_t stream);
+
+/* Row lookup: out[i] = scale * sum_j weight[i][j] * table[idx[i][j]], j < k (weight NULL: 1).  An index outside [0, rows) names no row.
+ * backward: dtable[rows, c] (all of it is written; NULL: not wanted) from the entries sorted by row and added in input order, without the row `padding`
+ * (-1: none); dweight[n, k] (NULL: not wanted; needs the table).  workspace: ls3d_embedding_workspace_bytes(n, k, c) bytes, 16-byte aligned.  n * k < 2^30. */
+int ls3d_embedding_forward(const void *table, long long table_ld, long long rows, int c, int dtype, const void *idx, int idx_dtype, int n, int k,
+                           const float *weight, float scale, void *out, ls3d_stream_t stream);
+size_t ls3d_embedding_workspace_bytes(int n, int k, int c);
+int ls3d_embedding_backward(const void *table, long long table_ld, long long rows, int c, int dtype, const void *idx, int idx_dtype, int n, int k,
+                            const float *weight, float scale, long long padding, const void *dout, long long dout_ld, void *dtable, float *dweight,
+                            void *workspace, size_t workspace_bytes, ls3d_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

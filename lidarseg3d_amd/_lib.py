@@ -25,6 +25,8 @@ EXPORTS = [
     "ls3d_seg_loss_workspace_bytes", "ls3d_seg_loss_saved_bytes", "ls3d_seg_loss_forward", "ls3d_seg_loss_backward", "ls3d_layer_norm_workspace_bytes", "ls3d_layer_norm_forward", "ls3d_layer_norm_backward", "ls3d_batch_norm_workspace_bytes", "ls3d_batch_norm_stats", "ls3d_batch_norm_finalize", "ls3d_batch_norm_apply", "ls3d_batch_norm_backward_sums", "ls3d_batch_norm_backward_apply", "ls3d_column_sums_workspace_bytes", "ls3d_column_sums", "ls3d_token_attention_forward", "ls3d_token_attention_workspace_bytes", "ls3d_token_attention_backward", "ls3d_devoxelize", "ls3d_devoxelize_grid", "ls3d_devoxelize_grid_workspace_bytes", "ls3d_interpolate_rows", "ls3d_interpolate_rows_backward", "ls3d_interpolate_rows_backward_workspace_bytes", "ls3d_grid_gather", "ls3d_nchw_to_nhwc", "ls3d_complete_concat", "ls3d_sfam", "ls3d_cross_attn", "ls3d_sffm_decoder", "ls3d_sffm_memory", "ls3d_sffm_memory_trace", "ls3d_stamp", "ls3d_points_cp", "ls3d_points_cuv",
     "ls3d_dynamic_point_to_voxel_workspace_bytes", "ls3d_dynamic_point_to_voxel_index", "ls3d_dynamic_point_to_voxel_forward", "ls3d_dynamic_point_to_voxel_backward",
     "ls3d_cyl_voxelize", "ls3d_unique_sorted_workspace_bytes", "ls3d_unique_sorted", "ls3d_dyn_point_features", "ls3d_act_affine", "ls3d_tta_merge",
+    "ls3d_dropout_forward", "ls3d_dropout_backward", "ls3d_residual_norm_forward", "ls3d_residual_norm_workspace_bytes", "ls3d_residual_norm_backward",
+    "ls3d_embedding_forward", "ls3d_embedding_workspace_bytes", "ls3d_embedding_backward",
 ]
 
 
@@ -83,6 +85,19 @@ class Sffm(ctypes.Structure):
                 ("w_in_planes", ctypes.c_void_p), ("pt_off", ctypes.c_void_p), ("gemm_products", ctypes.c_int32)]
 
 
+class Norm(ctypes.Structure):
+    """ls3d_norm_t"""
+    _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("kind", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """ls3d_residual_norm_t"""
+    _fields_ = [("in_", Norm), ("out", Norm), ("gate", ctypes.c_void_p), ("gate_ld", ctypes.c_longlong), ("state", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("stream_dtype", ctypes.c_int32), ("gate_kind", ctypes.c_int32), ("gate_dtype", ctypes.c_int32), ("alpha", ctypes.c_float), ("p", ctypes.c_float),
+                ("call", ctypes.c_uint32)]
+
+
 class LibraryMissing(RuntimeError):
     pass
 
@@ -97,7 +112,8 @@ def _configure(lib):
                  "ls3d_spconv_wgrad_workspace_bytes", "ls3d_spconv_pairs_bytes", "ls3d_tile_plan_bytes", "ls3d_column_sums_workspace_bytes", "ls3d_token_attention_workspace_bytes", "ls3d_tile_conv_packed_bytes", "ls3d_tile_conv_packed_bytes_bf16", "ls3d_tile_plan_workspace_bytes", "ls3d_radix_sort_workspace_bytes",
                  "ls3d_tile_conv_workspace_bytes", "ls3d_tile_conv_counter_bytes", "ls3d_tile_conv_trace_bytes", "ls3d_tile_chain_state_bytes", "ls3d_transvfe_planes_bytes", "ls3d_transvfe_workspace_bytes",
                  "ls3d_seg_loss_workspace_bytes", "ls3d_seg_loss_saved_bytes", "ls3d_layer_norm_workspace_bytes", "ls3d_batch_norm_workspace_bytes",
-                 "ls3d_dynamic_point_to_voxel_workspace_bytes", "ls3d_unique_sorted_workspace_bytes"):
+                 "ls3d_dynamic_point_to_voxel_workspace_bytes", "ls3d_unique_sorted_workspace_bytes",
+                 "ls3d_residual_norm_workspace_bytes", "ls3d_embedding_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
     for name in EXPORTS:
         fn = getattr(lib, name)  # AttributeError here = header/library mismatch: fail loudly

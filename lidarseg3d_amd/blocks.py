@@ -1,0 +1,281 @@
+"""Operators of a transformer block in training and serving: what stands between its matrix products and its attention.
+
+    from lidarseg3d_amd import blocks
+    rng = blocks.DropoutState(seed=0, device="cuda")
+    h = blocks.embedding(table, tokens, scale=32.0)                                             # lookup, gradient by sorted tokens
+    h, y = blocks.residual_norm(block(y), h, norm=blocks.Norm.of(ln), p=0.1, state=rng, return_sum=True)  # h + dropout(block), its norm
+    y = blocks.dropout(linear(y), 0.1, rng, relu=True)                                          # dropout(relu(.))
+    loss.backward(); rng.advance()
+
+All three take float32, bfloat16 and float16 tensors with any leading dimensions, run on the current stream of the tensors' device, allocate their
+outputs with torch and give the same bits for the same inputs.  Sums, statistics and parameter gradients are formed in 32 bits and rounded once.
+
+`use_in_training(model, rng)` puts the training forward of this package's models on them (counter-based dropout, residual and norm in one pass,
+camera sampling with a deterministic gradient)."""
+import torch
+from torch import nn
+
+from . import ops
+
+_KINDS = {"layer": 1, "rms": 2}
+
+
+class Norm(object):
+    """Norm("layer" | "rms", weight [c] or None, bias [c] or None, eps): what `norm` and `norm_in` of residual_norm take; Norm.of(module) for an
+    nn.LayerNorm / nn.RMSNorm over the last dimension"""
+
+    def __init__(self, kind, weight=None, bias=None, eps=1e-5):
+        if kind not in _KINDS:
+            raise ValueError("norm kind %r: 'layer' or 'rms'" % (kind,))
+        if not eps >= 0:
+            raise ValueError("eps %r" % (eps,))
+        self.kind, self.weight, self.bias, self.eps = kind, weight, bias, float(eps)
+
+    @classmethod
+    def of(cls, module):
+        if len(module.normalized_shape) != 1:
+            raise ValueError("a norm over the last dimension only is needed (normalized_shape %s)" % (tuple(module.normalized_shape),))
+        if isinstance(module, nn.LayerNorm):
+            return cls("layer", module.weight, module.bias, module.eps)
+        if isinstance(module, nn.RMSNorm):
+            if module.eps is None:  # torch's default there: the input type's eps
+                raise ValueError("nn.RMSNorm without an eps: give one")
+            return cls("rms", module.weight, None, module.eps)
+        raise TypeError("nn.LayerNorm or nn.RMSNorm needed, got %s" % type(module).__name__)
+
+
+class DropoutState(object):
+    """(seed, step) of a training program's dropout, on the device, and the number of the next call within the step.  The kernels read seed and step
+    when they run: a captured training step that ends with advance() draws new masks at every replay.  advance() comes after the backward pass
+    of everything drawn before it (an eager backward that finds another step raises, as after any in-place change of a saved tensor)."""
+
+    def __init__(self, seed, device="cuda", step=0):
+        self.tensor = torch.tensor([int(seed), int(step)], dtype=torch.int64, device=device)
+        self.calls = 0
+
+    def next_call(self):
+        n = self.calls
+        self.calls += 1
+        return n
+
+    def advance(self):
+        self.tensor[1:].add_(1)
+        self.calls = 0
+
+    def state_dict(self):
+        return {"state": self.tensor.clone(), "calls": self.calls}
+
+    def load_state_dict(self, sd):
+        self.tensor.copy_(sd["state"])
+        self.calls = int(sd["calls"])
+
+
+def _dtype_ok(t, what):
+    if t.dtype not in ops.DTYPES:
+        raise TypeError("%s: float32, bfloat16 or float16 needed, got %s" % (what, t.dtype))
+
+
+def _on_device(t, what):
+    if not (t.is_cuda or ops._SIM):
+        raise RuntimeError("%s: lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % (what, t.device))
+
+
+def _rows(t, c):
+    """t [..., c] as rows the kernels take: a view where the rows are contiguous, else a copy"""
+    r = t.reshape(-1, c) if c else t.reshape(0, 0)
+    if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < c):
+        r = r.contiguous()
+    return r
+
+
+def _draw(p, state, call):
+    """-> (p, state tensor, call) of a dropout"""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability %r" % (p,))
+    if p == 0.0:
+        return 0.0, None, 0
+    if isinstance(state, DropoutState):
+        call = state.next_call() if call is None else call
+        state = state.tensor
+    if not torch.is_tensor(state) or state.dtype != torch.int64 or state.shape != (2,) or not state.is_contiguous():
+        raise ValueError("dropout needs a DropoutState, or its int64 (seed, step) tensor")
+    if call is None:
+        raise ValueError("`call`, the number of this dropout within the step, is needed with a bare state tensor")
+    if not 0 <= int(call) < 1 << 32:
+        raise ValueError("call %r is not in [0, 2^32)" % (call,))
+    return p, state, int(call)
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, state, call, relu):
+        y = ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu).reshape(x.shape)
+        ctx.save_for_backward(state, y if relu else None)
+        ctx.args = (p, call, relu)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        state, y = ctx.saved_tensors
+        p, call, relu = ctx.args
+        c = dy.shape[-1]
+        dx = ops.dropout_backward(_rows(dy, c), y.reshape(-1, c) if relu else None, p, state, call, relu)
+        return dx.reshape(dy.shape), None, None, None, None
+
+
+def dropout(x, p, state, call=None, relu=False):
+    """dropout(x) - relu: dropout(relu(x)) - over the last dimension's rows, the mask made from (seed, step, call, row, column) in the forward pass and
+    again in the backward pass: nothing is stored (relu: the output itself, which the next layer keeps anyway, says where the gradient goes).
+    p is resolved to 1 / 65536 and what is kept is scaled by the inverse of the resolved probability.  state: a DropoutState, or its tensor together with
+    `call`; two dropouts of one step need different calls.  A dropped element is zero whatever stood there."""
+    _on_device(x, "dropout")
+    _dtype_ok(x, "dropout")
+    p, state, call = _draw(p, state, call)
+    if p == 0.0:
+        return torch.relu(x) if relu else x
+    if x.dim() == 0:
+        return dropout(x.reshape(1), p, state, call, relu).reshape(())
+    if x.numel() == 0:
+        return x
+    return _Dropout.apply(x, p, state, call, bool(relu))
+
+
+class Dropout(nn.Dropout):
+    """nn.Dropout on `dropout` with a DropoutState; evaluation passes its input through"""
+
+    def __init__(self, p, state):
+        super().__init__(p)
+        self.state = state
+
+    def forward(self, input):
+        return dropout(input, self.p, self.state) if self.training and self.p > 0 else input
+
+
+# ---------------------------------------------------------------------------------------------- residual, dropout, gate and norms
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gate, w_in, b_in, w_out, b_out, state, cfg):
+        kind_in, eps_in, kind_out, eps_out, alpha, p, call, want_sum = cfg
+        norms = ((kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None)
+        y, s, stats = ops.residual_norm_forward(x, residual, gate, norms[0], norms[1], alpha, p, state, call, want_sum)
+        ctx.save_for_backward(x, residual, gate, w_in, b_in, w_out, b_out, state, stats)
+        ctx.cfg = cfg
+        ctx.set_materialize_grads(False)
+        return (y, s) if kind_out and want_sum else (y if kind_out else s)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        x, residual, gate, w_in, b_in, w_out, b_out, state, stats = ctx.saved_tensors
+        kind_in, eps_in, kind_out, eps_out, alpha, p, call, want_sum = ctx.cfg
+        dy, ds = (grads if len(grads) == 2 else (grads[0], None)) if kind_out else (None, grads[0])
+        if dy is None and ds is None:
+            return (None,) * 9
+        c = x.shape[1]
+        out = ops.residual_norm_backward(x, residual, gate, (kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None,
+                                         alpha, p, state, call, stats, None if dy is None else _rows(dy, c), None if ds is None else _rows(ds, c), ctx.needs_input_grad[:7])
+        return (*out, None, None)
+
+
+def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.0, p=0.0, state=None, call=None, return_sum=False):
+    """One pass over a block's output x [..., c] and the residual stream:
+
+        t = norm_in(x);  s = alpha * residual + gate * dropout(t);  y = norm(s)      -> y;  (y, s) with return_sum;  s without a norm
+
+    norm / norm_in: a Norm (layer or RMS) or None.  gate: None, a single value, one per channel [c], or one per element (x's shape and type).
+    residual: x's shape, of x's type or float32 (s has its type).  p / state / call: as in `dropout`; p = 0 outside training.  c <= 8192."""
+    _on_device(x, "residual_norm")
+    _dtype_ok(x, "residual_norm")
+    if x.dim() < 1:
+        raise ValueError("residual_norm needs at least one dimension")
+    shape, c = x.shape, x.shape[-1]
+    if c > 8192:
+        raise ValueError("residual_norm takes rows of up to 8192 values, got %d" % c)
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(shape)))
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise TypeError("residual: %s or float32 needed, got %s" % (x.dtype, residual.dtype))
+    if gate is not None:
+        _dtype_ok(gate, "gate")
+        if gate.shape == shape and gate.dim() > 1:
+            if gate.dtype != x.dtype:
+                raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
+            gate = _rows(gate, c)
+        elif gate.numel() == 1 or gate.shape == (c,):
+            gate = gate.reshape(-1).expand(c).contiguous()
+        else:
+            raise ValueError("gate %s: one value, [%d] or %s" % (tuple(gate.shape), c, tuple(shape)))
+    params = []
+    for nm, what in ((norm_in, "norm_in"), (norm, "norm")):
+        if nm is not None and not isinstance(nm, Norm):
+            raise TypeError("%s: a blocks.Norm needed, got %s" % (what, type(nm).__name__))
+        for t, part in ((nm.weight, "weight"), (nm.bias, "bias")) if nm is not None else ((None, ""), (None, "")):
+            if t is not None:
+                _dtype_ok(t, "%s.%s" % (what, part))
+                if t.shape != (c,):
+                    raise ValueError("%s.%s %s: [%d] needed" % (what, part, tuple(t.shape), c))
+                t = t.contiguous()
+            params.append(t)
+    p, state, call = _draw(p, state, call)
+    x2, r2 = _rows(x, c), None if residual is None else _rows(residual, c)
+    kind_in, kind_out = _KINDS[norm_in.kind] if norm_in is not None else 0, _KINDS[norm.kind] if norm is not None else 0
+    eps_in, eps_out = norm_in.eps if norm_in is not None else 0.0, norm.eps if norm is not None else 0.0
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in [x2, r2, gate] + params):
+        res = _ResidualNorm.apply(x2, r2, gate, *params, state, (kind_in, eps_in, kind_out, eps_out, float(alpha), p, call, bool(return_sum)))
+    else:
+        y, s, _ = ops.residual_norm_forward(x2, r2, gate, (kind_in, params[0], params[1], eps_in) if kind_in else None,
+                                            (kind_out, params[2], params[3], eps_out) if kind_out else None, float(alpha), p, state, call, bool(return_sum), want_stats=False)
+        res = (y, s) if kind_out and return_sum else (y if kind_out else s)
+    return tuple(t.reshape(shape) for t in res) if isinstance(res, tuple) else res.reshape(shape)
+
+
+# ---------------------------------------------------------------------------------------------- row lookup
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, weight, idx, scale, padding):
+        ctx.save_for_backward(table, weight, idx)
+        ctx.args = (scale, padding)
+        return ops.embedding_forward(table, idx, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        table, weight, idx = ctx.saved_tensors
+        scale, padding = ctx.args
+        dt, dw = ops.embedding_backward(table, idx, weight, scale, padding, _rows(dout, dout.shape[-1]), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dt, dw, None, None, None
+
+
+def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
+    """scale * table[idx] of a table [rows, c]; idx int32 / int64 of any shape.  bag: the sum over idx's last dimension [..., k], with `weight` (float32, idx's
+    shape) the weighted sum, scale * sum_j weight[..., j] * table[idx[..., j]].  An index outside [0, rows) - -1 by custom - names no row: it reads as zero and takes no
+    gradient.  padding_idx: a row that is read but takes no gradient.  The table's gradient is dense; its entries are sorted by row and
+    added in input order: the same bits every time, for one frequent token as for many rare ones."""
+    _on_device(table, "embedding")
+    _dtype_ok(table, "embedding")
+    if table.dim() != 2:
+        raise ValueError("embedding: a table [rows, c] needed, got %s" % (tuple(table.shape),))
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise TypeError("embedding: int32 or int64 indices needed, got %s" % idx.dtype)
+    if weight is not None:
+        if weight.dtype != torch.float32:
+            raise TypeError("embedding: float32 weights needed, got %s" % weight.dtype)
+        if weight.shape != idx.shape or idx.dim() < 1:
+            raise ValueError("embedding: weights %s do not match the indices %s" % (tuple(weight.shape), tuple(idx.shape)))
+        bag = True
+    if bag and (idx.dim() < 1 or idx.shape[-1] == 0):
+        raise ValueError("embedding: no indices to sum over")
+    if padding_idx is not None and not -table.shape[0] <= padding_idx < table.shape[0]:
+        raise ValueError("padding_idx %r outside a table of %d rows" % (padding_idx, table.shape[0]))
+    padding = -1 if padding_idx is None else int(padding_idx) % table.shape[0]
+    lead, k = (idx.shape[:-1], idx.shape[-1]) if bag else (idx.shape, 1)
+    flat, tab, wgt = idx.reshape(-1, k).contiguous(), _rows(table, table.shape[1]), None if weight is None else weight.reshape(-1, k).contiguous()
+    if torch.is_grad_enabled() and (tab.requires_grad or (wgt is not None and wgt.requires_grad)):
+        out = _Embedding.apply(tab, wgt, flat, float(scale), padding)
+    else:
+        out = ops.embedding_forward(tab, flat, wgt, float(scale))
+    return out.reshape(*lead, table.shape[1])

@@ -1,0 +1,442 @@
+// resnorm.h — a transformer block's residual in one pass, forward and backward; instantiated per pair of element types by resnorm_*.hip.
+//
+//   t = N_in(x)                           N: layer norm, RMS norm or nothing; statistics and sums in f32
+//   d = keep ? t / (1 - p) : 0            counter-based mask (blocks_common.h)
+//   s = alpha * residual + gate * d       gate: one value per channel, per element, or none
+//   y = N_out(s)                          from s as it stands in registers: y does not see s's rounding to its type
+//
+// Backward, per row, with S the gradient that reaches s:
+//   u = dy * w_out;  S = ds + rstd (u - [mean u] - shat mean(u shat))        ([.]: layer norm only)
+//   dresidual = alpha S;  d gate = S d;  dt = keep ? gate S / (1 - p) : 0;  dx = N_in's gradient of dt, the same formula
+//   and the column sums  dw_out = sum dy shat, db_out = sum dy, dw_in = sum dt xhat, db_in = sum dt, dgate = sum S d.
+// s is computed again from x and the residual rather than kept: the forward's inputs are what autograd holds anyway.
+//
+// Bound by memory: x, residual (, gate) in and y (, s) out; backward dy (, ds) in addition, dx, dresidual out.  One pass: a row lives in the registers of
+// LPR lanes, VPT chunks of 8 columns each (LPR <= 64: 64 / LPR rows side by side in a wave, sums by lane exchange; LPR = 256: a row per
+// workgroup, sums through LDS).  Few lanes per row keep the exchanges few: 96 columns are 4 lanes x 3 chunks and two exchange steps a sum.
+#pragma once
+#include "blocks_common.h"
+
+struct ls3d_rn_args {
+  const void *x, *res, *gate;
+  size_t x_ld, res_ld, gate_ld;
+  int n, c;
+  int kind_in, kind_out, gate_kind;
+  const void *w_in, *b_in, *w_out, *b_out;
+  int w_in_t, b_in_t, w_out_t, b_out_t, gate_t;
+  float eps_in, eps_out, alpha, inv;
+  uint32_t thr, call;
+  const int64_t *state;
+  float *stats;  // [n][4]: mean, rstd of N_in, mean, rstd of N_out
+  void *y, *s;   // forward's outputs
+  const void *dy, *ds;
+  size_t dy_ld, ds_ld;
+  void *dx, *dres, *dgate;  // dgate: [n, c] of a full gate
+  float *partial;           // [blocks][columns' sums][c]
+  int nsum;                 // sums a block writes: the slots below that are wanted, packed
+  int slot[5];              // dw_out, db_out, dw_in, db_in, dgate (channel): place among the block's sums, -1: not wanted
+};
+
+// threads of a workgroup: 256, or the lanes of a row where that is more
+template <int LPR>
+constexpr int ls3d_rn_threads() { return LPR > 256 ? LPR : 256; }
+
+// sums of two values over the LPR lanes of a row; LPR > 64: over the workgroup (`lds`: 2 x 16 x 2 floats, halves used in turn so that one barrier a sum is enough)
+template <int LPR>
+struct ls3d_row_sums {
+  float *lds;
+  int turn;
+  __device__ __forceinline__ ls3d_row_sums(float *l) : lds(l), turn(0) {}
+  __device__ __forceinline__ void operator()(float &a, float &b) {
+#pragma unroll
+    for (int d = (LPR < 64 ? LPR : 64) / 2; d >= 1; d >>= 1) {
+      a += __shfl_xor(a, d);
+      b += __shfl_xor(b, d);
+    }
+    if (LPR > 64) {
+      float *half = lds + turn * 32;
+      if ((threadIdx.x & 63) == 0) { half[(threadIdx.x >> 6) * 2] = a; half[(threadIdx.x >> 6) * 2 + 1] = b; }
+      __syncthreads();
+      a = half[0];
+      b = half[1];
+#pragma unroll
+      for (int w = 1; w < LPR / 64; ++w) { a += half[2 * w]; b += half[2 * w + 1]; }
+      turn ^= 1;
+    }
+  }
+  __device__ __forceinline__ void operator()(float &a) {
+    if (LPR > 64) {
+      float b = 0.0f;
+      (*this)(a, b);
+      return;
+    }
+#pragma unroll
+    for (int d = (LPR < 64 ? LPR : 64) / 2; d >= 1; d >>= 1) a += __shfl_xor(a, d);
+  }
+};
+
+// mean and 1 / sqrt(variance + eps) of a row's values (two passes over registers: no cancellation); RMS: mean 0.  Columns behind the row's end hold zeros;
+// m0: live columns from the lane's first chunk on
+template <int LPR, int VPT>
+__device__ __forceinline__ void ls3d_rn_stats(const float (&v)[VPT][8], int kind, int m0, float inv_c, float eps, ls3d_row_sums<LPR> &sums, float &mean, float &rstd) {
+  mean = 0.0f;
+  if (kind == LS3D_NORM_LAYER) {
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a = fmaf(v[i][j], inv_c, a);  // shares of the mean: a row of the type's lowest values does not overflow
+    sums(a);
+    mean = a;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int m = m0 - i * LPR * 8;
+    if (m >= 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = v[i][j] - mean;
+        q = fmaf(d, d, q);
+      }
+    } else if (m > 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = j < m ? v[i][j] - mean : 0.0f;
+        q = fmaf(d, d, q);
+      }
+    }
+  }
+  sums(q);
+  rstd = 1.0f / sqrtf(q * inv_c + eps);
+}
+
+// FULL: a norm before or a gate; without them neither their registers nor their sums exist
+template <typename TX, typename TR, int LPR, int VPT, bool FULL>
+__global__ __launch_bounds__(ls3d_rn_threads<LPR>()) void k_resnorm_fwd(const ls3d_rn_args A) {
+  __shared__ float s_sum[64];
+  constexpr int ROWS = ls3d_rn_threads<LPR>() / LPR;
+  const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR, c = A.c;
+  const float inv_c = 1.0f / (float)c;
+  ls3d_dropout_key key = {};
+  if (A.thr) key = ls3d_dropout_key_load(A.state, A.call);
+  ls3d_row_sums<LPR> sums(s_sum);
+  float wo[VPT][8], bo[VPT][8], wi[FULL ? VPT : 1][8], bi[FULL ? VPT : 1][8], g[FULL ? VPT : 1][8];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (lane + i * LPR) * 8;
+    ls3d_param8(A.w_out, A.w_out_t, col, c, 1.0f, wo[i]);
+    ls3d_param8(A.b_out, A.b_out_t, col, c, 0.0f, bo[i]);
+    if (FULL) {
+      ls3d_param8(A.w_in, A.w_in_t, col, c, 1.0f, wi[i]);
+      ls3d_param8(A.b_in, A.b_in_t, col, c, 0.0f, bi[i]);
+      ls3d_param8(A.gate_kind == LS3D_GATE_CHANNEL ? A.gate : nullptr, A.gate_t, col, c, 1.0f, g[i]);
+    }
+  }
+  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < A.n; row0 += (long long)gridDim.x * ROWS) {  // the same trips for every lane of a wave / workgroup
+    const bool live = row0 + sub < A.n;
+    const size_t row = (size_t)(live ? row0 + sub : A.n - 1);
+    int m0 = live ? c - lane * 8 : 0;  // a dead row reads the last one and counts as zeros
+    LS3D_OPAQUE(m0);
+    ls3d_raw8<TX> rx[VPT], rg[FULL ? VPT : 1];
+    ls3d_raw8<TR> rr[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) rx[i] = ls3d_load8<TX>((const TX *)A.x + row * A.x_ld, (lane + i * LPR) * 8, c);
+    if (A.res) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) rr[i] = ls3d_load8<TR>((const TR *)A.res + row * A.res_ld, (lane + i * LPR) * 8, c);
+    }
+    if (FULL && A.gate_kind == LS3D_GATE_FULL) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) rg[i] = ls3d_load8<TX>((const TX *)A.gate + row * A.gate_ld, (lane + i * LPR) * 8, c);
+    }
+    float v[VPT][8];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) ls3d_unpack8<TX>(rx[i], m0 - i * LPR * 8, v[i]);
+    float st[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (FULL && A.kind_in) {
+      ls3d_rn_stats<LPR, VPT>(v, A.kind_in, m0, inv_c, A.eps_in, sums, st[0], st[1]);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - st[0]) * st[1], wi[i][j], bi[i][j]);  // (behind the end: weight and bias are zero)
+    }
+    if (A.thr) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const uint32_t keep = ls3d_keep8(key, (uint32_t)(lane + i * LPR), (uint32_t)row, A.thr);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = ((keep >> j) & 1u) ? v[i][j] * A.inv : 0.0f;
+      }
+    }
+    if (FULL && A.gate_kind) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        if (A.gate_kind == LS3D_GATE_FULL) ls3d_unpack8<TX>(rg[i], m0 - i * LPR * 8, g[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= g[i][j];
+      }
+    }
+    if (A.res) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float r[8];
+        ls3d_unpack8<TR>(rr[i], m0 - i * LPR * 8, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf(A.alpha, r[j], v[i][j]);
+      }
+    }
+    if (A.s) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) ls3d_store8<TR>((TR *)A.s + row * c + (lane + i * LPR) * 8, v[i], m0 - i * LPR * 8);
+    }
+    if (A.kind_out) {
+      ls3d_rn_stats<LPR, VPT>(v, A.kind_out, m0, inv_c, A.eps_out, sums, st[2], st[3]);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf((v[i][j] - st[2]) * st[3], wo[i][j], bo[i][j]);
+        ls3d_store8<TX>((TX *)A.y + row * c + (lane + i * LPR) * 8, o, m0 - i * LPR * 8);
+      }
+    }
+    if (A.stats && live && lane == 0) *(float4 *)(A.stats + row * 4) = make_float4(st[0], st[1], st[2], st[3]);
+  }
+}
+
+template <typename TX, typename TR, int LPR, int VPT, bool FULL>
+__global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_resnorm_bwd(const ls3d_rn_args A) {
+  constexpr int THREADS = ls3d_rn_threads<LPR>(), ROWS = THREADS / LPR, WIDTH = LPR * VPT * 8, NV = FULL ? VPT : 1, NSUM = FULL ? 5 : 2;
+  __shared__ float s_sum[64];
+  __shared__ float s_col[LPR <= 64 ? 4 * WIDTH : 1];
+  const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR, c = A.c;
+  const float inv_c = 1.0f / (float)c;
+  ls3d_dropout_key key = {};
+  if (A.thr) key = ls3d_dropout_key_load(A.state, A.call);
+  ls3d_row_sums<LPR> sums(s_sum);
+  float acc[NSUM][VPT][8], wo[VPT][8], wi[NV][8], bi[NV][8], g[NV][8];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int col = (lane + i * LPR) * 8;
+#pragma unroll
+    for (int k = 0; k < NSUM; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[k][i][j] = 0.0f;
+    ls3d_param8(A.w_out, A.w_out_t, col, c, 1.0f, wo[i]);
+    if (FULL) {
+      ls3d_param8(A.w_in, A.w_in_t, col, c, 1.0f, wi[i]);
+      ls3d_param8(A.b_in, A.b_in_t, col, c, 0.0f, bi[i]);
+      ls3d_param8(A.gate_kind == LS3D_GATE_CHANNEL ? A.gate : nullptr, A.gate_t, col, c, 1.0f, g[i]);
+    }
+  }
+  for (long long row0 = (long long)blockIdx.x * ROWS; row0 < A.n; row0 += (long long)gridDim.x * ROWS) {
+    const bool live = row0 + sub < A.n;
+    const size_t row = (size_t)(live ? row0 + sub : A.n - 1);
+    int m0 = live ? c - lane * 8 : 0;
+    LS3D_OPAQUE(m0);
+    ls3d_raw8<TX> rx[VPT], ry[VPT], rg[NV];
+    ls3d_raw8<TR> rr[VPT], rs[VPT];
+    // every load of the row before the first use of one
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) rx[i] = ls3d_load8<TX>((const TX *)A.x + row * A.x_ld, (lane + i * LPR) * 8, c);
+    if (A.res) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) rr[i] = ls3d_load8<TR>((const TR *)A.res + row * A.res_ld, (lane + i * LPR) * 8, c);
+    }
+    if (A.dy) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) ry[i] = ls3d_load8<TX>((const TX *)A.dy + row * A.dy_ld, (lane + i * LPR) * 8, c);
+    }
+    if (A.ds) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) rs[i] = ls3d_load8<TR>((const TR *)A.ds + row * A.ds_ld, (lane + i * LPR) * 8, c);
+    }
+    if (FULL && A.gate_kind == LS3D_GATE_FULL) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) rg[i] = ls3d_load8<TX>((const TX *)A.gate + row * A.gate_ld, (lane + i * LPR) * 8, c);
+    }
+    const float4 st = *(const float4 *)(A.stats + row * 4);
+    float xh[NV][8], sh[VPT][8], S[VPT][8];
+    uint32_t keep[VPT];
+    // s again, as the forward pass computed it
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      ls3d_unpack8<TX>(rx[i], m0 - i * LPR * 8, sh[i]);
+      if (FULL) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          xh[i][j] = A.kind_in ? (sh[i][j] - st.x) * st.y : sh[i][j];
+          sh[i][j] = A.kind_in ? fmaf(xh[i][j], wi[i][j], bi[i][j]) : xh[i][j];
+        }
+      }
+      keep[i] = 0xFFu;
+      if (A.thr) {
+        keep[i] = ls3d_keep8(key, (uint32_t)(lane + i * LPR), (uint32_t)row, A.thr);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sh[i][j] = ((keep[i] >> j) & 1u) ? sh[i][j] * A.inv : 0.0f;
+      }
+      if (FULL) {
+        if (A.gate_kind == LS3D_GATE_FULL) ls3d_unpack8<TX>(rg[i], m0 - i * LPR * 8, g[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sh[i][j] *= g[i][j];
+      }
+      if (A.res) {
+        float r[8];
+        ls3d_unpack8<TR>(rr[i], m0 - i * LPR * 8, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sh[i][j] = fmaf(A.alpha, r[j], sh[i][j]);
+      }
+    }
+    // the gradient of s
+    if (A.dy) {
+      float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        ls3d_unpack8<TX>(ry[i], m0 - i * LPR * 8, S[i]);  // zeros behind the row's end keep what stands there out of every sum
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sh[i][j] = (sh[i][j] - st.z) * st.w;
+          acc[0][i][j] = fmaf(S[i][j], sh[i][j], acc[0][i][j]);
+          acc[1][i][j] += S[i][j];
+          S[i][j] *= wo[i][j];
+          s1 += S[i][j];
+          s2 = fmaf(S[i][j], sh[i][j], s2);
+        }
+      }
+      sums(s1, s2);
+      const float c1 = A.kind_out == LS3D_NORM_LAYER ? s1 * inv_c : 0.0f, c2 = s2 * inv_c;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) S[i][j] = st.w * (S[i][j] - c1 - sh[i][j] * c2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) S[i][j] = 0.0f;
+    }
+    if (A.ds) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float d[8];
+        ls3d_unpack8<TR>(rs[i], m0 - i * LPR * 8, d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) S[i][j] += d[j];
+      }
+    }
+    if (A.dres) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = A.alpha * S[i][j];
+        ls3d_store8<TR>((TR *)A.dres + row * c + (lane + i * LPR) * 8, o, m0 - i * LPR * 8);
+      }
+    }
+    if (FULL && A.gate_kind) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float o[8];
+        LS3D_OPAQUE(keep[i]);  // (the dropped t is formed again from xh: kept from above it would be 8 more registers a chunk)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float d = ((keep[i] >> j) & 1u) ? (A.kind_in ? fmaf(xh[i][j], wi[i][j], bi[i][j]) : xh[i][j]) * A.inv : 0.0f;
+          o[j] = S[i][j] * d;
+          S[i][j] *= g[i][j];
+        }
+        if (A.gate_kind == LS3D_GATE_FULL) {
+          if (A.dgate) ls3d_store8<TX>((TX *)A.dgate + row * c + (lane + i * LPR) * 8, o, m0 - i * LPR * 8);
+        } else if (m0 - i * LPR * 8 > 0) {  // (S is not zero behind the row's end; columns there are never stored, a dead row's must not be added)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[4][i][j] += o[j];
+        }
+      }
+    }
+    if (A.thr) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        LS3D_OPAQUE(keep[i]);  // (lane masks of its bits are made again rather than parked)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) S[i][j] = ((keep[i] >> j) & 1u) ? S[i][j] * A.inv : 0.0f;  // dt
+      }
+    }
+    if (FULL && A.kind_in) {
+      float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const bool in = m0 - i * LPR * 8 > 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (in) {
+            acc[2][i][j] = fmaf(S[i][j], xh[i][j], acc[2][i][j]);
+            acc[3][i][j] += S[i][j];
+          }
+          S[i][j] *= wi[i][j];  // zero behind the row's end
+          s1 += S[i][j];
+          s2 = fmaf(S[i][j], xh[i][j], s2);
+        }
+      }
+      sums(s1, s2);
+      const float c1 = A.kind_in == LS3D_NORM_LAYER ? s1 * inv_c : 0.0f, c2 = s2 * inv_c;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) S[i][j] = st.y * (S[i][j] - c1 - xh[i][j] * c2);
+    }
+    if (A.dx) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) ls3d_store8<TX>((TX *)A.dx + row * c + (lane + i * LPR) * 8, S[i], m0 - i * LPR * 8);
+    }
+  }
+  // the block's column sums: the row groups of a wave by lane exchange, the four waves through LDS in order; a fixed tree, no atomics
+#pragma unroll
+  for (int k = 0; k < NSUM; ++k) {
+    if (A.slot[k] < 0) continue;
+    float *__restrict__ dst = A.partial + ((size_t)blockIdx.x * A.nsum + A.slot[k]) * c;
+    if (LPR > 64) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) ls3d_store8<float>(dst + (lane + i * LPR) * 8, acc[k][i], c - (lane + i * LPR) * 8);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float a = acc[k][i][j];
+#pragma unroll
+        for (int d = LPR; d < 64; d <<= 1) a += __shfl_xor(a, d);
+        if ((threadIdx.x & 63) < LPR) s_col[(threadIdx.x >> 6) * WIDTH + (lane + i * LPR) * 8 + j] = a;
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < c; i += THREADS) dst[i] = (s_col[i] + s_col[WIDTH + i]) + (s_col[2 * WIDTH + i] + s_col[3 * WIDTH + i]);
+    __syncthreads();
+  }
+}
+
+// lanes per row and chunks per lane (the rule that picks one: rn_shape in resnorm.hip)
+#define LS3D_RN_SIMPLE(GO) GO(4, 1) GO(4, 2) GO(4, 3) GO(8, 2) GO(16, 2) GO(32, 2) GO(64, 2) GO(256, 1) GO(256, 2) GO(512, 2)
+#define LS3D_RN_FULL(GO) GO(4, 1) GO(8, 1) GO(16, 1) GO(32, 1) GO(64, 1) GO(256, 1) GO(512, 1) GO(1024, 1)
+
+template <typename TX, typename TR>
+static bool ls3d_rn_launch_types(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {
+#define LS3D_RN_GO(L_, V_, F_)                                                                                                                             \
+  if (lpr == L_ && vpt == V_) {                                                                                                                            \
+    if (fwd) hipLaunchKernelGGL((k_resnorm_fwd<TX, TR, L_, V_, F_>), dim3((unsigned)blocks), dim3(ls3d_rn_threads<L_>()), 0, stream, a);                   \
+    else hipLaunchKernelGGL((k_resnorm_bwd<TX, TR, L_, V_, F_>), dim3((unsigned)blocks), dim3(ls3d_rn_threads<L_>()), 0, stream, a);                       \
+    return true;                                                                                                                                           \
+  }
+#define LS3D_RN_GO_SIMPLE(L_, V_) LS3D_RN_GO(L_, V_, false)
+#define LS3D_RN_GO_FULL(L_, V_) LS3D_RN_GO(L_, V_, true)
+  if (full) { LS3D_RN_FULL(LS3D_RN_GO_FULL) }
+  else { LS3D_RN_SIMPLE(LS3D_RN_GO_SIMPLE) }
+#undef LS3D_RN_GO_FULL
+#undef LS3D_RN_GO_SIMPLE
+#undef LS3D_RN_GO
+  return false;
+}
+
+bool ls3d_rn_launch_f32(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream);
+bool ls3d_rn_launch_bf16(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream);
+bool ls3d_rn_launch_f16(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream);
+bool ls3d_rn_launch_bf16_f32(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream);
+bool ls3d_rn_launch_f16_f32(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream);

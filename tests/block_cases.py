@@ -1,0 +1,445 @@
+"""Shared by test_blocks_hipsim.py (kernel logic on the host) and test_blocks_gpu.py: the training-block operators (lidarseg3d_amd/blocks.py) against
+plain implementations in 64 bits, with error bounds that follow from the arithmetic.
+
+A result is off by its own rounding, half a step of its type (u = eps / 2 of the value), and by what 32-bit arithmetic does before: each 32-bit operation
+is off by 2^-24 of its result, a sum of up to 8192 values is 32 additions a lane and a tree of 8 (40 steps), and at most three such sums are nested.
+(40 * 3 + a handful of products) < 128, so the bound is u |ref| + 128 * 2^-24 * scale, `scale` being the largest magnitude that enters the
+subtractions on the way; it is computed beside the reference.  Column sums over n rows add at most ceil(n / blocks) + 64 terms in sequence."""
+import numpy as np
+import torch
+
+K32 = 128 * 2.0 ** -24
+
+
+def philox_words(c0, c1, c2, c3, k0, k1):
+    """Philox4x32, 10 rounds, on Python integers: the definition, one counter at a time"""
+    x, k = [c0, c1, c2, c3], [k0, k1]
+    for _ in range(10):
+        a, b = x[0] * 0xD2511F53, x[2] * 0xCD9E8D57
+        x = [(b >> 32) ^ x[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ x[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return x
+
+
+def keep_mask(rows, c, p, seed, step, call):
+    """[rows, c] truth values, and the factor of what is kept (numpy, vectorised over the counters)"""
+    u = np.uint64
+    g = (c + 7) // 8
+    x = [np.tile(np.arange(g, dtype=u), (rows, 1)), np.tile(np.arange(rows, dtype=u)[:, None], (1, g)), np.full((rows, g), call, u),
+         np.full((rows, g), step % 2 ** 32, u)]
+    k0, k1 = seed % 2 ** 32, (seed >> 32) % 2 ** 32
+    for _ in range(10):
+        a, b = x[0] * u(0xD2511F53), x[2] * u(0xCD9E8D57)
+        x = [(b >> u(32)) ^ x[1] ^ u(k0), b & u(0xFFFFFFFF), (a >> u(32)) ^ x[3] ^ u(k1), a & u(0xFFFFFFFF)]
+        k0, k1 = (k0 + 0x9E3779B9) % 2 ** 32, (k1 + 0xBB67AE85) % 2 ** 32
+    draws = np.stack([(w >> u(s)) & u(0xFFFF) for w in x for s in (0, 16)], -1).reshape(rows, 8 * g)[:, :c]
+    t = int(np.floor(65536 * float(np.float32(p)) + 0.5))
+    return torch.from_numpy(np.ascontiguousarray(draws >= t)), (65536.0 / (65536 - t) if t < 65536 else 0.0)
+
+
+def unit(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check(got, ref, scale, what="", k=K32):
+    """|got - ref| <= u |ref| + k * scale, element by element (scale broadcasts); half a smallest step besides, for values below the normal range"""
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    if ref.numel() == 0:
+        return
+    g = got.detach().cpu().double()
+    assert torch.equal(torch.isnan(g), torch.isnan(ref)), what + ": NaN in other places"
+    bound = unit(got.dtype) * ref.abs() + k * torch.as_tensor(scale, dtype=torch.float64) + torch.finfo(got.dtype).tiny * unit(got.dtype) * 2
+    bad = (g - ref).abs() - bound
+    bad = torch.where(torch.isnan(ref) | (g == ref), torch.full_like(bad, -1.0), bad)
+    i = int(bad.argmax())
+    assert float(bad.max()) <= 0, "%s: element %d is %.9g, reference %.9g, bound %.3g" % (what, i, float(g.reshape(-1)[i]), float(ref.reshape(-1)[i]),
+                                                                                        float(bound.expand_as(ref).reshape(-1)[i]))
+
+
+def _rmax(t):
+    return t.abs().amax(1, keepdim=True)
+
+
+def _norm(v, kind, w, b, eps):
+    """-> value, hat, 1 / std in float64"""
+    m = v.mean(1, keepdim=True) if kind == "layer" else torch.zeros_like(v[:, :1])
+    r = 1.0 / ((v - m).square().mean(1, keepdim=True) + eps).sqrt()
+    h = (v - m) * r
+    y = h * w if w is not None else h
+    return (y + b if b is not None else y), h, r
+
+
+def _back(u, h, r, kind):
+    g = u - h * (u * h).mean(1, keepdim=True)
+    return r * (g - u.mean(1, keepdim=True)) if kind == "layer" else r * g
+
+
+def residual_norm_reference(x, residual, norm, norm_in, gate, alpha, p, draw, dy, ds):
+    """every output of residual_norm and every gradient by the formulas, in float64 on the host: name -> (reference, scale).  norm / norm_in:
+    None or (kind, weight, bias, eps) of host tensors; draw: (seed, step, call); dy / ds: gradients or None"""
+    D = lambda t: None if t is None else t.detach().cpu().double()
+    x, residual, gate, dy, ds = D(x), D(residual), D(gate), D(dy), D(ds)
+    w_in, b_in = (D(norm_in[1]), D(norm_in[2])) if norm_in else (None, None)
+    w_out, b_out = (D(norm[1]), D(norm[2])) if norm else (None, None)
+    mag = lambda t, other: other if t is None else float(t.abs().max())
+    res = {}
+    t, T = x, _rmax(x)
+    if norm_in:
+        t, xh, r_in = _norm(x, norm_in[0], w_in, b_in, norm_in[3])
+        cond_in = T * r_in
+        T = cond_in * (1 + _rmax(xh)) * mag(w_in, 1.0) + mag(b_in, 0.0)
+    keep, inv = keep_mask(x.shape[0], x.shape[1], p, *draw) if p > 0 else (torch.ones(x.shape, dtype=torch.bool), 1.0)
+    d = torch.where(keep, t * inv, torch.zeros(1, dtype=torch.float64))
+    T = T * inv
+    g = gate if gate is not None else torch.ones(1, dtype=torch.float64)
+    gmax = float(g.abs().max())
+    s = g * d + (alpha * residual if residual is not None else 0.0)
+    Ss = gmax * T + (abs(alpha) * _rmax(residual) if residual is not None else 0.0)
+    res["s"] = (s, Ss)
+    G = torch.zeros_like(s)
+    Gs = torch.zeros_like(Ss)
+    if norm:
+        y, sh, r_out = _norm(s, norm[0], w_out, b_out, norm[3])
+        cond = Ss * r_out
+        Hs = cond * (1 + _rmax(sh))
+        res["y"] = (y, Hs * mag(w_out, 1.0) + mag(b_out, 0.0))
+        if dy is not None:
+            u = dy * w_out if w_out is not None else dy
+            G = _back(u, sh, r_out, norm[0])
+            Gs = r_out * _rmax(u) * (1 + _rmax(sh)) * (1 + Hs)
+            res["w_out"], res["b_out"] = ((dy * sh).sum(0), (_rmax(dy) * Hs).sum()), (dy.sum(0), dy.abs().sum(0))
+    if ds is not None:
+        G, Gs = G + ds, Gs + _rmax(ds)
+    if dy is None and ds is None:
+        return res
+    res["residual"] = (alpha * G, abs(alpha) * Gs)
+    if gate is not None:
+        res["gate"] = (G * d, Gs * T) if gate.dim() == 2 else ((G * d).sum(0), (Gs * T).sum())
+    dt = torch.where(keep, g * G * inv, torch.zeros(1, dtype=torch.float64))
+    Dt = gmax * Gs * inv
+    if norm_in:
+        res["w_in"], res["b_in"] = ((dt * xh).sum(0), (Dt * (1 + cond_in)).sum()), (dt.sum(0), Dt.sum())
+        u = dt * w_in if w_in is not None else dt
+        res["x"] = (_back(u, xh, r_in, norm_in[0]), r_in * Dt * mag(w_in, 1.0) * (1 + _rmax(xh)) * (1 + cond_in * (1 + _rmax(xh))))
+    else:
+        res["x"] = (dt, Dt)
+    return res
+
+
+def embedding_reference(table, idx, weight, scale, padding, dy, bag):
+    """(out, scale), (dtable, scale), (dweight, scale) in float64, entry by entry in input order"""
+    t, g = table.detach().cpu().double(), dy.detach().cpu().double()
+    c, rows = t.shape[1], t.shape[0]
+    ix = idx.cpu().long().reshape(-1, idx.shape[-1] if bag else 1)
+    n, k = ix.shape
+    w = weight.detach().cpu().double().reshape(n, k) if weight is not None else torch.ones(n, k, dtype=torch.float64)
+    g = g.reshape(n, c)
+    out, out_s = torch.zeros(n, c, dtype=torch.float64), torch.zeros(n, c, dtype=torch.float64)
+    dt, dt_s = torch.zeros_like(t), torch.zeros_like(t)
+    dw, dw_s = torch.zeros(n, k, dtype=torch.float64), torch.zeros(n, k, dtype=torch.float64)
+    for j in range(k):
+        hit = torch.nonzero((ix[:, j] >= 0) & (ix[:, j] < rows))[:, 0]
+        v = ix[hit, j]
+        term = scale * w[hit, j].unsqueeze(1) * t[v]
+        out[hit] += term
+        out_s[hit] += term.abs()
+        dw[hit, j], dw_s[hit, j] = scale * (t[v] * g[hit]).sum(1), abs(scale) * (t[v] * g[hit]).abs().sum(1)
+        if padding is not None:
+            hit = hit[v != padding]
+            v = ix[hit, j]
+        term = scale * w[hit, j].unsqueeze(1) * g[hit]
+        dt.index_add_(0, v, term)
+        dt_s.index_add_(0, v, term.abs())
+    return (out, out_s), (dt, dt_s), (dw, dw_s)
+
+
+# ---------------------------------------------------------------------------------------------- sizes and forms
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+# rows, c, x type, stream type, norm, norm_in, gate, alpha, p, return_sum: one token, one column, widths of every shape rule (4 / 16 / 64 / 256 lanes), odd and
+# even, either side of each border, rows that leave lanes and workgroups idle
+RESIDUAL_NORM = [
+    (1, 1, F32, F32, "layer", None, None, 1.0, 0.0, False),
+    (3, 7, F32, F32, "rms", "layer", "full", 1.5, 0.3, True),
+    (70, 8, BF16, BF16, "layer", None, "channel", 1.0, 0.5, True),
+    (66, 33, F16, F16, "layer", "rms", None, 0.5, 0.1, False),
+    (131, 96, F32, F32, "layer", None, None, 1.0, 0.1, False),
+    (9, 96, BF16, F32, None, "layer", "channel", 1.0, 0.25, True),
+    (17, 128, F16, F32, "rms", "rms", "full", 1.0, 0.0, True),
+    (20, 129, F32, F32, "rms", None, "channel", -1.0, 0.2, True),
+    (18, 257, BF16, F32, "layer", "layer", None, 1.0, 0.1, True),
+    (5, 512, F16, F16, "rms", None, "scalar", 2.0, 0.9, False),
+    (6, 513, F32, F32, "layer", "rms", "channel", 1.0, 0.1, True),
+    (4, 771, F16, F16, "layer", None, "full", 1.25, 0.2, True),
+    (3, 1536, BF16, BF16, "rms", "rms", None, 1.0, 0.0, True),
+    (5, 2047, BF16, F32, "layer", None, None, 1.0, 0.1, False),
+    (3, 2049, F32, F32, "layer", "layer", "full", 1.0, 0.1, True),
+    (1, 4096, BF16, BF16, "rms", None, None, 1.0, 0.0, True),
+    (2, 6145, F16, F32, "rms", "layer", "channel", 0.5, 0.1, True),
+    (2, 8192, BF16, BF16, "layer", None, None, 1.0, 0.4, False),
+]
+
+# rows, c, type, p, relu
+DROPOUT = [(1, 1, F32, 0.5, False), (68, 96, F32, 0.1, False), (5, 7, BF16, 0.3, True), (33, 192, F32, 0.1, True), (11, 1001, BF16, 0.25, False), (3, 4099, F16, 0.9, True),
+           (4, 64, F16, 1.0, False), (1, 5000, F32, 0.05, False), (7, 8, BF16, 1e-4, False)]
+
+# table rows, c, type, index shape, bag, weights, scale, how the tokens fall
+EMBEDDING = [
+    (5, 1, F32, (1,), False, False, 1.0, "uniform"),
+    (7, 9, BF16, (3, 5), False, False, 2.0, "uniform"),
+    (40, 96, F32, (200,), False, False, 1.0, "uniform"),
+    (3, 64, F32, (500,), False, False, 1.0, "few"),
+    (1, 17, F16, (333,), False, False, 0.5, "few"),
+    (1000, 33, F16, (257,), False, False, 1.0, "uniform"),
+    (50, 48, F32, (60, 8), True, True, 1.0, "holes"),
+    (30, 130, BF16, (40, 3), True, True, 4.0, "holes"),
+    (30, 24, F32, (2, 9, 3), True, False, 1.0, "holes"),
+    (70000, 5, F32, (90,), False, False, 1.0, "uniform"),
+    (12, 1030, BF16, (70,), False, False, 32.0, "few"),
+    (9, 64, F32, (1300,), False, False, 1.0, "one"),
+]
+
+
+def tensor(gen, *shape, dtype=F32, scale=1.0, shift=0.0, device="cpu"):
+    return (torch.randn(*shape, generator=gen) * scale + shift).to(dtype).to(device)
+
+
+def indices(gen, rows, shape, how, device, dtype=torch.int64):
+    if how == "one":
+        ix = torch.full(shape, rows - 1)
+    elif how == "few":
+        ix = torch.randint(0, min(rows, 3), shape, generator=gen)
+    else:
+        ix = torch.randint(0, rows, shape, generator=gen)
+    if how == "holes":  # rows that name nothing, and some beyond either end of the table
+        ix = torch.where(torch.rand(shape, generator=gen) < 0.4, torch.full(shape, -1), ix)
+        ix.reshape(-1)[0], ix.reshape(-1)[1] = rows, -7
+        ix[1] = -1
+    return ix.to(dtype).to(device)
+
+
+def run_residual_norm(case, device, seed=0):
+    """one case forward and backward through blocks.residual_norm, checked against the formulas"""
+    from lidarseg3d_amd import blocks
+    n, c, T, R, kind, kind_in, gate_kind, alpha, p, want_sum = case
+    gen = torch.Generator().manual_seed(seed + n * 131 + c)
+    mk = lambda *s, **kw: tensor(gen, *s, device=device, **kw).requires_grad_()
+    x, res = mk(n, c, dtype=T), mk(n, c, dtype=R, scale=2.0)
+    norm = (kind, mk(c, dtype=R, scale=0.1, shift=1.0), mk(c, dtype=T, scale=0.1) if kind == "layer" else None, 1e-5) if kind else None
+    norm_in = (kind_in, mk(c, dtype=T, scale=0.1, shift=1.0), mk(c, scale=0.1) if kind_in == "layer" else None, 1e-6) if kind_in else None
+    gate = {None: None, "full": lambda: mk(n, c, dtype=T), "channel": lambda: mk(c, dtype=R), "scalar": lambda: mk(1, dtype=F32)}[gate_kind]
+    gate = gate() if gate else None
+    state = blocks.DropoutState(0x123456789ABCDEF + seed, device=device, step=5)
+    state.calls = 7
+    mod = lambda m: blocks.Norm(m[0], m[1], m[2], m[3]) if m else None
+    out = blocks.residual_norm(x, res, norm=mod(norm), norm_in=mod(norm_in), gate=gate, alpha=alpha, p=p, state=state, return_sum=want_sum)
+    y, s = (out if want_sum else (out, None)) if kind else (None, out)
+    dy = tensor(gen, n, c, dtype=T, device=device) if y is not None else None
+    ds = tensor(gen, n, c, dtype=R, device=device) if s is not None else None
+    leaves = dict(x=x, residual=res)
+    for nm, tag in ((norm, "out"), (norm_in, "in")):
+        if nm:
+            leaves["w_" + tag] = nm[1]
+            if nm[2] is not None:
+                leaves["b_" + tag] = nm[2]
+    if gate is not None:
+        leaves["gate"] = gate
+    grads = torch.autograd.grad([t for t in (y, s) if t is not None], list(leaves.values()), [t for t in (dy, ds) if t is not None])
+    ref = residual_norm_reference(x, res, norm, norm_in, gate.detach().expand(c) if gate_kind == "scalar" else gate, alpha, p, (0x123456789ABCDEF + seed, 5, 7), dy, ds)
+    if y is not None:
+        check(y, *ref["y"], what="y")
+    if s is not None:
+        check(s, *ref["s"], what="s")
+    for name, g in zip(leaves, grads):
+        r, sc = ref[name]
+        if name == "gate" and gate_kind == "scalar":  # autograd adds the c channel gradients up, each rounded to f32
+            r, sc = r.sum().reshape(1), sc * c
+        check(g, r, sc, what="d " + name)
+
+
+def run_dropout(case, device, seed=0):
+    from lidarseg3d_amd import blocks
+    n, c, T, p, relu = case
+    gen = torch.Generator().manual_seed(seed + n + c)
+    x = tensor(gen, n, c, dtype=T, device=device)
+    if x.numel() > 20:
+        x.reshape(-1)[::9] = float("nan")  # behind the mask nothing of it is seen
+        x.reshape(-1)[1::9] = float("inf")
+    x.requires_grad_()
+    dy = tensor(gen, n, c, dtype=T, device=device)
+    state = blocks.DropoutState(-5 - seed, device=device, step=2 ** 32 + 3)
+    y = blocks.dropout(x, p, state, call=9, relu=relu)
+    (dx,) = torch.autograd.grad(y, [x], [dy])
+    keep, inv = keep_mask(n, c, p, (-5 - seed) % 2 ** 64, 3, 9)
+    zero = torch.zeros(1, dtype=torch.float64)
+    xd = x.detach().cpu().double()
+    want = torch.where(keep, (torch.relu(xd) if relu else xd) * inv, zero)
+    got = y.detach().cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got) & torch.isinf(want), torch.isinf(want))
+    fin = torch.isfinite(want)
+    # one product in f32 by a factor that is itself rounded to f32, then the rounding to the type
+    check(torch.where(fin.to(y.device), y.detach(), torch.zeros_like(y)), torch.where(fin, want, zero), torch.where(fin, want, zero).abs(), what="y")
+    live = keep & ~(xd <= 0) if relu else keep
+    ref = torch.where(live, dy.cpu().double() * inv, zero)
+    check(dx, ref, ref.abs(), what="dx")
+
+
+def run_embedding(case, device, seed=0, index=torch.int64):
+    from lidarseg3d_amd import blocks
+    rows, c, T, shape, bag, weights, scale, how = case
+    gen = torch.Generator().manual_seed(seed + rows + c)
+    table = tensor(gen, rows, c, dtype=T, device=device).requires_grad_()
+    idx = indices(gen, rows, shape, how, device, index)
+    weight = torch.rand(shape, generator=gen).to(device).requires_grad_() if weights else None
+    padding = rows // 2 if how == "uniform" and rows > 20 else None
+    y = blocks.embedding(table, idx, weight=weight, scale=scale, padding_idx=padding, bag=bag)
+    assert y.shape == (*(shape[:-1] if bag else shape), c)
+    dy = tensor(gen, *y.shape, dtype=T, device=device)
+    grads = torch.autograd.grad(y, [table] + ([weight] if weights else []), [dy])
+    out, dt, dw = embedding_reference(table, idx, weight, scale, padding, dy, bag)
+    check(y.reshape(-1, c), *out, what="out")
+    # a row's entries: <= `tile` in sequence, then a partial sum a tile
+    check(grads[0], *dt, what="dtable", k=(np.prod(shape) + 16) * 2.0 ** -24)
+    if weights:
+        check(grads[1].reshape(dw[0].shape), *dw, what="dweight")
+    again = torch.autograd.grad(blocks.embedding(table, idx, weight=weight, scale=scale, padding_idx=padding, bag=bag), [table], [dy])[0]
+    assert torch.equal(again, grads[0])
+
+
+def run_strides_and_absent_parts(device):
+    """leading dimensions, column slices, transposed and expanded tensors, empty tensors; norms without weights, no residual, outputs that nothing uses"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(11)
+    wide = tensor(gen, 6, 40, device=device)
+    x = wide[:, 5:24]  # rows 40 apart that start anywhere
+    res = tensor(gen, 19, 6, device=device).t()  # columns contiguous
+    y, s = blocks.residual_norm(x, res, norm=blocks.Norm("layer"), return_sum=True)
+    ref = residual_norm_reference(x, res, ("layer", None, None, 1e-5), None, None, 1.0, 0.0, None, None, None)
+    check(y, *ref["y"], what="y of a slice")
+    check(s, *ref["s"], what="s of a slice")
+    x3 = tensor(gen, 2, 3, 19, device=device)
+    y3 = blocks.residual_norm(x3, norm=blocks.Norm("rms"))
+    ref = residual_norm_reference(x3.reshape(6, 19), None, ("rms", None, None, 1e-5), None, None, 1.0, 0.0, None, None, None)
+    assert y3.shape == x3.shape
+    check(y3.reshape(6, 19), *ref["y"], what="y of [2, 3, 19]")
+    # a norm without parameters, its output unused: only the sum's gradient arrives; an expanded gradient (of .sum())
+    x4, r4 = x3.clone().requires_grad_(), tensor(gen, 2, 3, 19, device=device).requires_grad_()
+    w = torch.ones(19, device=device, requires_grad=True)
+    y4, s4 = blocks.residual_norm(x4, r4, norm=blocks.Norm("layer", w), alpha=0.5, return_sum=True)
+    dx, dr, dw = torch.autograd.grad(s4.sum(), [x4, r4, w])
+    assert bool((dx == 1).all()) and bool((dr == 0.5).all()) and bool((dw == 0).all())
+    dx, = torch.autograd.grad(blocks.residual_norm(x4, r4, norm=blocks.Norm("layer", w)).sum(), [x4])
+    ref = residual_norm_reference(x4.reshape(6, 19), r4.reshape(6, 19), ("layer", w, None, 1e-5), None, None, 1.0, 0.0, None, torch.ones(6, 19), None)
+    check(dx.reshape(6, 19), *ref["x"], what="dx of a summed norm")
+    # no norm at all: the residual sum alone; nothing to differentiate; 1-D input
+    z = blocks.residual_norm(x3, x3, alpha=2.0)
+    check(z.reshape(6, 19), x3.cpu().double().reshape(6, 19) * 3, x3.cpu().double().reshape(6, 19).abs() * 3, what="plain sum")
+    assert blocks.residual_norm(x3[0, 0], norm=blocks.Norm("rms")).shape == (19,)
+    # empty tensors, both ways
+    e = torch.zeros(0, 24, device=device, requires_grad=True)
+    w24 = torch.ones(24, device=device, requires_grad=True)
+    ye = blocks.residual_norm(e, e, norm=blocks.Norm("layer", w24))
+    ge, gw = torch.autograd.grad(ye, [e, w24], [torch.zeros(0, 24, device=device)])
+    assert ye.shape == (0, 24) and ge.shape == (0, 24) and bool((gw == 0).all())
+    st = blocks.DropoutState(3, device=device)
+    assert blocks.dropout(e, 0.5, st).shape == (0, 24)
+    assert blocks.dropout(x3, 0.0, None) is x3 and bool((blocks.dropout(x3, 0.0, None, relu=True) == torch.relu(x3)).all())
+    # dropout of a slice equals the slice's copy: the mask goes by row and column, not by address
+    assert torch.equal(blocks.dropout(x, 0.4, st.tensor, call=1), blocks.dropout(x.contiguous(), 0.4, st.tensor, call=1))
+    # tables and gradients with strides; an empty batch and a table nobody names
+    tab = tensor(gen, 9, 40, device=device)[:, 3:20].requires_grad_()
+    ix = torch.tensor([[0, 8], [3, 3]], device=device)
+    out = blocks.embedding(tab, ix)
+    assert torch.equal(out, tab[ix])
+    g = tensor(gen, 2, 17, 2, device=device).transpose(1, 2)
+    (dt,) = torch.autograd.grad(out, [tab], [g])
+    want = torch.zeros(9, 17, dtype=torch.float64).index_add_(0, ix.cpu().reshape(-1), g.cpu().double().reshape(-1, 17))
+    check(dt, want, want.abs(), what="dtable")
+    t0 = torch.ones(4, 8, device=device, requires_grad=True)
+    o0 = blocks.embedding(t0, torch.zeros(0, dtype=torch.int32, device=device))
+    assert o0.shape == (0, 8) and bool((torch.autograd.grad(o0, [t0], [torch.zeros(0, 8, device=device)])[0] == 0).all())
+    on = blocks.embedding(t0, torch.full((5,), -1, device=device))
+    assert bool((on == 0).all()) and bool((torch.autograd.grad(on.sum(), [t0])[0] == 0).all())
+
+
+def run_masked_rows(device):
+    """everything dropped, rows of equal values, rows of the type's lowest value, infinities in dropped places"""
+    from lidarseg3d_amd import blocks
+    st = blocks.DropoutState(1, device=device)
+    b = torch.arange(16.0, device=device)
+    x = torch.full((3, 16), float("inf"), device=device).requires_grad_()
+    y, s = blocks.residual_norm(x, torch.zeros(3, 16, device=device), norm=blocks.Norm("layer", None, b), p=1.0, state=st, return_sum=True)
+    assert bool((s == 0).all()) and torch.equal(y, b.expand(3, 16))  # variance 0: the bias is left
+    (dx,) = torch.autograd.grad([y, s], [x], [torch.ones_like(y), torch.ones_like(s)])
+    assert bool((dx == 0).all())
+    for T in (torch.float16, torch.bfloat16):  # their sum is beyond float32 for bf16
+        lo = torch.full((2, 64), torch.finfo(T).min, dtype=T, device=device)
+        y = blocks.residual_norm(lo, norm=blocks.Norm("layer"))
+        assert bool((y == 0).all())  # all values alike: deviation 0
+    r = blocks.residual_norm(torch.full((2, 64), 60000.0, dtype=torch.float16, device=device), norm=blocks.Norm("rms"))
+    assert bool(((r.float() - 1).abs() <= 2.0 ** -11).all())
+    # a NaN stays in its row
+    z = torch.ones(3, 16, device=device)
+    z[1, 2] = float("nan")
+    y = blocks.residual_norm(z, norm=blocks.Norm("rms"))
+    assert bool(torch.isnan(y[1]).all()) and not bool(torch.isnan(y[0]).any()) and not bool(torch.isnan(y[2]).any())
+    # p = 1 of a bare dropout; relu keeps NaN like torch.relu
+    assert bool((blocks.dropout(x, 1.0, st) == 0).all())
+    # NaN in a table row nobody names, in a weight of an index that names none
+    t = torch.ones(3, 4, device=device)
+    t[1] = float("nan")
+    w = torch.tensor([[1.0, float("nan")]], device=device)
+    assert bool((blocks.embedding(t, torch.tensor([[0, -1]], device=device), weight=w) == 1).all())
+
+
+def block_parameters(gen, width, table, device, dtype=torch.float32):
+    mk = lambda *s, **k: tensor(gen, *s, dtype=dtype, device=device, **k).requires_grad_()
+    return dict(table=mk(table, width), gate=mk(width, scale=0.5, shift=0.5), w1=mk(2 * width, width, scale=width ** -0.5), w2=mk(width, 2 * width, scale=(2 * width) ** -0.5),
+                n1=mk(width, scale=0.1, shift=1.0), n2=mk(width, scale=0.1, shift=1.0), b2=mk(width, scale=0.1))
+
+
+def block_forward(P, tokens, state, p):
+    """embedding -> RMS norm before the block -> linear, dropout(relu), linear -> norm after it, gate, scaled residual, LayerNorm"""
+    from lidarseg3d_amd import blocks
+    F = torch.nn.functional
+    h = blocks.embedding(P["table"], tokens, scale=2.0)
+    y = blocks.residual_norm(h, norm=blocks.Norm("rms", P["n1"]))
+    y = F.linear(blocks.dropout(F.linear(y, P["w1"]), p, state, relu=True), P["w2"])
+    return blocks.residual_norm(y, h, norm=blocks.Norm("layer", P["n2"], P["b2"]), norm_in=blocks.Norm("rms", P["n1"]), gate=P["gate"], alpha=0.5, p=p, state=state,
+                                return_sum=True)
+
+
+def run_block(device, rows, width, table):
+    """the operators together, as a block uses them: outputs against float64, every gradient against the float64 graph and against differences of it"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(rows)
+    P = block_parameters(gen, width, table, device)
+    tokens = indices(gen, table, (rows,), "few", device)
+    state = blocks.DropoutState(17, device=device, step=1)
+    p = 0.25
+    y, s = block_forward(P, tokens, state, p)
+    assert state.calls == 2
+    dy, ds = tensor(gen, rows, width, device=device), tensor(gen, rows, width, device=device)
+    grads = torch.autograd.grad([y, s], list(P.values()), [dy, ds])
+    # the same block in float64 with the masks of the definition
+    k1, inv = keep_mask(rows, 2 * width, p, 17, 1, 0)
+    k2, _ = keep_mask(rows, width, p, 17, 1, 1)
+
+    def plain(Q):
+        rms = lambda v, w: v * torch.rsqrt(v.square().mean(1, keepdim=True) + 1e-5) * w
+        h = 2.0 * Q["table"][tokens.cpu()]
+        m = (torch.relu(rms(h, Q["n1"]) @ Q["w1"].t()) * k1 * inv) @ Q["w2"].t()
+        t = 0.5 * h + Q["gate"] * (rms(m, Q["n1"]) * k2 * inv)
+        d = t - t.mean(1, keepdim=True)
+        return d * torch.rsqrt(d.square().mean(1, keepdim=True) + 1e-5) * Q["n2"] + Q["b2"], t
+    Q = {k: v.detach().cpu().double().requires_grad_() for k, v in P.items()}
+    yr, sr = plain(Q)
+    want = torch.autograd.grad([yr, sr], list(Q.values()), [dy.cpu().double(), ds.cpu().double()])
+    # products of `width` / 2 width terms in 32 bits come in between: K32 with the largest value of the tensor as scale, 8-fold for the five operators in a row
+    for name, g, w in [("y", y, yr), ("s", s, sr)] + [("d " + n, g, w) for n, g, w in zip(P, grads, want)]:
+        check(g, w.detach(), float(w.detach().abs().max()), what=name, k=8 * K32)
+    # differences of the float64 block along a random direction: the derivative is the gradients' product with it
+    dirs = {k: torch.randn(v.shape, generator=gen, dtype=torch.float64) for k, v in Q.items()}
+    val = lambda e: sum(float((o * w.cpu().double()).sum()) for o, w in zip(plain({k: Q[k].detach() + e * dirs[k] for k in Q}), (dy, ds)))
+    slope, along = (val(1e-6) - val(-1e-6)) / 2e-6, sum(float((g.cpu().double() * dirs[k]).sum()) for k, g in zip(Q, grads))
+    assert abs(slope - along) <= 1e-4 * sum(float((g.cpu().double() * dirs[k]).abs().sum()) for k, g in zip(Q, grads))
