@@ -82,10 +82,20 @@ def _on_device(t, what):
 
 def _rows(t, c):
     """t [..., c] as rows the kernels take: a view where the rows are contiguous, else a copy"""
-    r = t.reshape(-1, c) if c else t.reshape(0, 0)
+    r = t if t.dim() == 2 else t.reshape(-1, c) if c else t.reshape(0, 0)
     if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < c):
         r = r.contiguous()
     return r
+
+
+def _shaped(t, shape):
+    return t if t.shape == shape else t.reshape(shape)
+
+
+def _once(what):
+    """a second derivative would come out as a constant: refuse it (the check of torch's once_differentiable at a tenth of its cost)"""
+    if torch.is_grad_enabled():
+        raise RuntimeError("%s is differentiable once (backward with create_graph=True)" % what)
 
 
 def _draw(p, state, call):
@@ -111,19 +121,19 @@ def _draw(p, state, call):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, state, call, relu):
-        y = ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu).reshape(x.shape)
+        y = _shaped(ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu), x.shape)
         ctx.save_for_backward(state, y if relu else None)
         ctx.args = (p, call, relu)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("dropout")
         state, y = ctx.saved_tensors
         p, call, relu = ctx.args
         c = dy.shape[-1]
-        dx = ops.dropout_backward(_rows(dy, c), y.reshape(-1, c) if relu else None, p, state, call, relu)
-        return dx.reshape(dy.shape), None, None, None, None
+        dx = ops.dropout_backward(_rows(dy, c), _rows(y, c) if relu else None, p, state, call, relu)
+        return _shaped(dx, dy.shape), None, None, None, None
 
 
 def dropout(x, p, state, call=None, relu=False):
@@ -167,8 +177,8 @@ class _ResidualNorm(torch.autograd.Function):
         return (y, s) if kind_out and want_sum else (y if kind_out else s)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
+        _once("residual_norm")
         x, residual, gate, w_in, b_in, w_out, b_out, state, stats = ctx.saved_tensors
         kind_in, eps_in, kind_out, eps_out, alpha, p, call, want_sum = ctx.cfg
         dy, ds = (grads if len(grads) == 2 else (grads[0], None)) if kind_out else (None, grads[0])
@@ -206,7 +216,7 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
                 raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
             gate = _rows(gate, c)
         elif gate.numel() == 1 or gate.shape == (c,):
-            gate = gate.reshape(-1).expand(c).contiguous()
+            gate = (gate if gate.shape == (c,) else gate.reshape(1).expand(c)).contiguous()
         else:
             raise ValueError("gate %s: one value, [%d] or %s" % (tuple(gate.shape), c, tuple(shape)))
     params = []
@@ -230,7 +240,7 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
         y, s, _ = ops.residual_norm_forward(x2, r2, gate, (kind_in, params[0], params[1], eps_in) if kind_in else None,
                                             (kind_out, params[2], params[3], eps_out) if kind_out else None, float(alpha), p, state, call, bool(return_sum), want_stats=False)
         res = (y, s) if kind_out and return_sum else (y if kind_out else s)
-    return tuple(t.reshape(shape) for t in res) if isinstance(res, tuple) else res.reshape(shape)
+    return tuple(_shaped(t, shape) for t in res) if isinstance(res, tuple) else _shaped(res, shape)
 
 
 # ---------------------------------------------------------------------------------------------- row lookup
@@ -242,8 +252,8 @@ class _Embedding(torch.autograd.Function):
         return ops.embedding_forward(table, idx, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _once("embedding")
         table, weight, idx = ctx.saved_tensors
         scale, padding = ctx.args
         dt, dw = ops.embedding_backward(table, idx, weight, scale, padding, _rows(dout, dout.shape[-1]), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
@@ -278,4 +288,4 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
         out = _Embedding.apply(tab, wgt, flat, float(scale), padding)
     else:
         out = ops.embedding_forward(tab, flat, wgt, float(scale))
-    return out.reshape(*lead, table.shape[1])
+    return out if len(lead) == 1 else out.reshape(*lead, table.shape[1])

@@ -111,33 +111,47 @@ __global__ __launch_bounds__(256) void k_emb_tiles(const uint32_t *__restrict__ 
   }
 }
 
-// a wave for each tile in which a row begins that goes on in the next one: partial[j][1] + partial[j + 1][0] + ... while the tiles begin with that row
+// a workgroup for each tile in which a row begins that goes on in the next one: partial[j][1] + partial[j + 1][0] + ... while the tiles begin with that row.
+// `lpr` lanes per partial row, the 256 / lpr groups take the tiles in turn (one wave walking the 700 tiles of a row one after the other took 210 us), their
+// sums are added in order.
 template <typename T>
-__global__ __launch_bounds__(64) void k_emb_join(const uint32_t *__restrict__ keys, int entries, int tile, int ntiles, long long rows, int c, float scale,
-                                                 const float *__restrict__ partial, T *__restrict__ dtable) {
-  const int j = (int)blockIdx.x, lane = (int)threadIdx.x;
-  if (j + 1 >= ntiles) return;
+__global__ __launch_bounds__(256) void k_emb_join(const uint32_t *__restrict__ keys, int entries, int tile, int ntiles, int lpr, long long rows, int c, float scale,
+                                                  const float *__restrict__ partial, T *__restrict__ dtable) {
+  __shared__ float s_sum[256][9];
+  const int j = (int)blockIdx.x;
   const long long hi = (long long)(j + 1) * tile;
   const uint32_t cur = keys[hi - 1];
-  if (cur >= (uint32_t)rows || keys[hi] != cur) return;  // nothing goes on
+  if (cur >= (uint32_t)rows || keys[hi] != cur) return;  // nothing goes on (uniform over the workgroup, like the next line)
   if (j > 0 && keys[hi - tile] == cur && keys[hi - tile - 1] == cur) return;  // it began in an earlier tile
-  int last = j + 1;  // the last tile that begins with this row
+  int last = j + 1;  // the last tile that begins with this row: sorted keys, so those that do are the first of any run of tiles
   for (;;) {
-    const long long t = (long long)last + 1 + lane;
-    const unsigned long long on = __ballot(t < ntiles && keys[t * tile < entries ? t * tile : 0] == cur);
-    const int run = on == ~0ull ? 64 : __ffsll((long long)~on) - 1;
-    last += run;
-    if (run < 64) break;
+    const long long t = (long long)last + 1 + threadIdx.x;
+    const int on = __syncthreads_count(t < ntiles && keys[t < ntiles ? t * tile : 0] == cur);
+    last += on;
+    if (on < 256) break;
   }
-  for (int col = ((int)blockIdx.y * 64 + lane) * 8; col < c; col += (int)gridDim.y * 512) {
-    const int m = c - col;
-    float acc[8], p[8];
-    ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)j * 2 + 1) * c, col, c), m, acc);
-    for (int t = j + 1; t <= last; ++t) {
+  const int lane = (int)threadIdx.x % lpr, grp = (int)threadIdx.x / lpr, ngrp = 256 / lpr;
+  const int col = ((int)blockIdx.y * lpr + lane) * 8, m = c - col;
+  float acc[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
+  if (m > 0) {
+#pragma unroll 4
+    for (int t = j + 1 + grp; t <= last; t += ngrp) {
+      float p[8];
       ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)t * 2) * c, col, c), m, p);
 #pragma unroll
       for (int q = 0; q < 8; ++q) acc[q] += p[q];
     }
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) s_sum[threadIdx.x][q] = acc[q];
+  __syncthreads();
+  if (grp == 0 && m > 0) {
+    ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)j * 2 + 1) * c, col, c), m, acc);
+    for (int g = 0; g < ngrp; ++g)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] += s_sum[g * lpr + lane][q];
 #pragma unroll
     for (int q = 0; q < 8; ++q) acc[q] *= scale;
     ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
@@ -250,8 +264,8 @@ extern "C" int ls3d_embedding_backward(const void *table, long long table_ld, lo
       EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_tiles<T>), grid, dim3(256), 0, stream, (const uint32_t *)skeys, (const int32_t *)order, entries, tile, lpr, rows, c, k, weight,
                                           scale, (const T *)dout, (size_t)dout_ld, (T *)dtable, partial));
       if (ntiles > 1)
-        EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)ntiles, (unsigned)((groups + 63) / 64)), dim3(64), 0, stream, (const uint32_t *)skeys, entries, tile,
-                                            ntiles, rows, c, scale, (const float *)partial, (T *)dtable));
+        EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)(ntiles - 1), grid.y), dim3(256), 0, stream, (const uint32_t *)skeys, entries, tile,
+                                            ntiles, lpr, rows, c, scale, (const float *)partial, (T *)dtable));
     }
   }
   LS3D_RETURN_IF_LAUNCH_FAILED();

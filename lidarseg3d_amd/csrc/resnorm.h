@@ -57,6 +57,7 @@ struct ls3d_row_sums {
       float *half = lds + turn * 32;
       if ((threadIdx.x & 63) == 0) { half[(threadIdx.x >> 6) * 2] = a; half[(threadIdx.x >> 6) * 2 + 1] = b; }
       __syncthreads();
+      half += (threadIdx.x / LPR) * (LPR / 64) * 2;  // the waves of this thread's row
       a = half[0];
       b = half[1];
 #pragma unroll
@@ -208,7 +209,8 @@ template <typename TX, typename TR, int LPR, int VPT, bool FULL>
 __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_resnorm_bwd(const ls3d_rn_args A) {
   constexpr int THREADS = ls3d_rn_threads<LPR>(), ROWS = THREADS / LPR, WIDTH = LPR * VPT * 8, NV = FULL ? VPT : 1, NSUM = FULL ? 5 : 2;
   __shared__ float s_sum[64];
-  __shared__ float s_col[LPR <= 64 ? 4 * WIDTH : 1];
+  constexpr int PARTS = LPR <= 64 ? 4 : ROWS;  // row groups that meet in LDS: the waves (their own groups by lane exchange), or the rows of a workgroup
+  __shared__ float s_col[PARTS > 1 ? PARTS * WIDTH : 1];
   const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR, c = A.c;
   const float inv_c = 1.0f / (float)c;
   ls3d_dropout_key key = {};
@@ -388,12 +390,12 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_r
       for (int i = 0; i < VPT; ++i) ls3d_store8<TX>((TX *)A.dx + row * c + (lane + i * LPR) * 8, S[i], m0 - i * LPR * 8);
     }
   }
-  // the block's column sums: the row groups of a wave by lane exchange, the four waves through LDS in order; a fixed tree, no atomics
+  // the block's column sums: the row groups of a wave by lane exchange, what is left through LDS in order; a fixed tree, no atomics
 #pragma unroll
   for (int k = 0; k < NSUM; ++k) {
     if (A.slot[k] < 0) continue;
     float *__restrict__ dst = A.partial + ((size_t)blockIdx.x * A.nsum + A.slot[k]) * c;
-    if (LPR > 64) {
+    if (PARTS == 1) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) ls3d_store8<float>(dst + (lane + i * LPR) * 8, acc[k][i], c - (lane + i * LPR) * 8);
       continue;
@@ -405,17 +407,22 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_r
         float a = acc[k][i][j];
 #pragma unroll
         for (int d = LPR; d < 64; d <<= 1) a += __shfl_xor(a, d);
-        if ((threadIdx.x & 63) < LPR) s_col[(threadIdx.x >> 6) * WIDTH + (lane + i * LPR) * 8 + j] = a;
+        if (LPR > 64 || (threadIdx.x & 63) < LPR) s_col[(LPR > 64 ? sub : threadIdx.x >> 6) * WIDTH + (lane + i * LPR) * 8 + j] = a;
       }
     __syncthreads();
-    for (int i = threadIdx.x; i < c; i += THREADS) dst[i] = (s_col[i] + s_col[WIDTH + i]) + (s_col[2 * WIDTH + i] + s_col[3 * WIDTH + i]);
+    for (int i = threadIdx.x; i < c; i += THREADS) {
+      float s = s_col[i];
+#pragma unroll
+      for (int q = 1; q < PARTS; ++q) s += s_col[q * WIDTH + i];
+      dst[i] = s;
+    }
     __syncthreads();
   }
 }
 
 // lanes per row and chunks per lane (the rule that picks one: rn_shape in resnorm.hip)
-#define LS3D_RN_SIMPLE(GO) GO(4, 1) GO(4, 2) GO(4, 3) GO(8, 2) GO(16, 2) GO(32, 2) GO(64, 2) GO(256, 1) GO(256, 2) GO(512, 2)
-#define LS3D_RN_FULL(GO) GO(4, 1) GO(8, 1) GO(16, 1) GO(32, 1) GO(64, 1) GO(256, 1) GO(512, 1) GO(1024, 1)
+#define LS3D_RN_SIMPLE(GO) GO(4, 1) GO(4, 2) GO(4, 3) GO(8, 2) GO(16, 2) GO(32, 2) GO(64, 2) GO(128, 2) GO(256, 2) GO(512, 2)
+#define LS3D_RN_FULL(GO) GO(4, 1) GO(8, 1) GO(16, 1) GO(32, 1) GO(64, 1) GO(128, 1) GO(256, 1) GO(512, 1) GO(1024, 1)
 
 template <typename TX, typename TR>
 static bool ls3d_rn_launch_types(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {

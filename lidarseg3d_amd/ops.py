@@ -1844,22 +1844,45 @@ def _row_view(t, name):
         return None, 0
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         raise RuntimeError("%s: 2-D tensor with contiguous rows needed (shape %s, strides %s)" % (name, tuple(t.shape), t.stride()))
-    return _vp_any(t), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    _device_ok(t)
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _device_ok(t):
+    if t.is_cuda == _SIM:
+        raise RuntimeError("hipsim test hook active: CPU tensors only" if _SIM else
+                           "lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % t.device)
+
+
+def _addr(t):
+    """data pointer of a contiguous tensor (None stays None) as a plain integer, for the entry points whose argument types _lib declares"""
+    if t is None:
+        return None
+    if not t.is_contiguous():
+        raise RuntimeError("non-contiguous tensor passed to libls3d")
+    _device_ok(t)
+    return t.data_ptr()
 
 
 def _same_device(ref, *others):
+    dev = ref.device
     for t in others:
-        if t is not None and t.device != ref.device:
-            raise RuntimeError("tensors on different devices: %s and %s" % (ref.device, t.device))
+        if t is not None and t.device != dev:
+            raise RuntimeError("tensors on different devices: %s and %s" % (dev, t.device))
 
 
 def _call_on(t, fn, what, *args):
     """the C call with the tensor's device current (a launch on another device's stream would fail) and on its current stream"""
-    if not t.is_cuda or t.device.index == torch.cuda.current_device():
-        check(fn(*args, _stream(t)), what)
-        return
-    with torch.cuda.device(t.device):
-        check(fn(*args, _stream(t)), what)
+    dev = t.get_device()
+    if dev < 0:
+        rc = fn(*args, None)
+    elif dev == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
 
 
 def dropout_forward(x, p, state, call, relu=False):
@@ -1867,8 +1890,8 @@ def dropout_forward(x, p, state, call, relu=False):
     _same_device(x, state)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     px, ld = _row_view(x, "x")
-    _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ctypes.c_longlong(ld), ctypes.c_longlong(x.shape[0]), ctypes.c_longlong(x.shape[1]),
-             DTYPES[x.dtype], ctypes.c_float(p), _ptr(state), ctypes.c_uint32(call), int(relu), _ptr(y))
+    _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ld, x.shape[0], x.shape[1],
+             DTYPES[x.dtype], p, _addr(state), call, int(relu), _addr(y))
     return y
 
 
@@ -1877,8 +1900,8 @@ def dropout_backward(dy, y, p, state, call, relu=False):
     _same_device(dy, state, y)
     dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
     pd, ld = _row_view(dy, "dy")
-    _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ctypes.c_longlong(ld), _ptr(y), ctypes.c_longlong(dy.shape[0]),
-             ctypes.c_longlong(dy.shape[1]), DTYPES[dy.dtype], ctypes.c_float(p), _ptr(state), ctypes.c_uint32(call), int(relu), _ptr(dx))
+    _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ld, _addr(y), dy.shape[0],
+             dy.shape[1], DTYPES[dy.dtype], p, _addr(state), call, int(relu), _addr(dx))
     return dx
 
 
@@ -1889,19 +1912,19 @@ def residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, ca
         if nm is not None:
             dst.kind, dst.eps = nm[0], nm[3]
             if nm[1] is not None:
-                dst.weight, dst.weight_dtype = _ptr(nm[1]), DTYPES[nm[1].dtype]
+                dst.weight, dst.weight_dtype = _addr(nm[1]), DTYPES[nm[1].dtype]
             if nm[2] is not None:
-                dst.bias, dst.bias_dtype = _ptr(nm[2]), DTYPES[nm[2].dtype]
+                dst.bias, dst.bias_dtype = _addr(nm[2]), DTYPES[nm[2].dtype]
     if gate is not None:
         d.gate_dtype = DTYPES[gate.dtype]
         if gate.dim() == 1:
-            d.gate_kind, d.gate, d.gate_ld = 1, _ptr(gate), 0
+            d.gate_kind, d.gate, d.gate_ld = 1, _addr(gate), 0
         else:
             d.gate_kind = 2
             d.gate, d.gate_ld = _row_view(gate, "gate")
     d.dtype, d.stream_dtype = DTYPES[x.dtype], DTYPES[(x if residual is None else residual).dtype]
     d.alpha, d.p, d.call = alpha, p, call
-    d.state = _ptr(state)
+    d.state = _addr(state)
     return d
 
 
@@ -1915,8 +1938,8 @@ def residual_norm_forward(x, residual=None, gate=None, norm_in=None, norm_out=No
     stats = torch.empty((n, 4), dtype=torch.float32, device=x.device) if want_stats else None
     px, x_ld = _row_view(x, "x")
     pr, r_ld = _row_view(residual, "residual")
-    _call_on(x, _L().ls3d_residual_norm_forward, "ls3d_residual_norm_forward", px, ctypes.c_longlong(x_ld), pr, ctypes.c_longlong(r_ld), n, c, ctypes.byref(d),
-             _ptr(y), _ptr(s), _ptr(stats))
+    _call_on(x, _L().ls3d_residual_norm_forward, "ls3d_residual_norm_forward", px, x_ld, pr, r_ld, n, c, ctypes.byref(d),
+             _addr(y), _addr(s), _addr(stats))
     return y, s, stats
 
 
@@ -1931,9 +1954,8 @@ def residual_norm_backward(x, residual, gate, norm_in, norm_out, alpha, p, state
     L = _L()
     ws = _ws(L.ls3d_residual_norm_workspace_bytes(n, c), x)
     (px, x_ld), (pr, r_ld), (py, y_ld), (ps, s_ld) = _row_view(x, "x"), _row_view(residual, "residual"), _row_view(dy, "dy"), _row_view(ds, "ds")
-    ll = ctypes.c_longlong
-    _call_on(x, L.ls3d_residual_norm_backward, "ls3d_residual_norm_backward", px, ll(x_ld), pr, ll(r_ld), n, c, ctypes.byref(d), _ptr(stats), py, ll(y_ld), ps, ll(s_ld),
-             *[_ptr(g) for g in grads], _ptr(ws), ctypes.c_size_t(ws.numel()))
+    _call_on(x, L.ls3d_residual_norm_backward, "ls3d_residual_norm_backward", px, x_ld, pr, r_ld, n, c, ctypes.byref(d), _addr(stats), py, y_ld, ps, s_ld,
+             *[_addr(g) for g in grads], _addr(ws), ws.numel())
     return grads
 
 
@@ -1943,8 +1965,8 @@ def embedding_forward(table, idx, weight=None, scale=1.0):
     (n, k), c = idx.shape, table.shape[1]
     out = torch.empty((n, c), dtype=table.dtype, device=table.device)
     pt, ld = _row_view(table, "table")
-    _call_on(table, _L().ls3d_embedding_forward, "ls3d_embedding_forward", pt, ctypes.c_longlong(ld), ctypes.c_longlong(table.shape[0]), c, DTYPES[table.dtype], _ptr(idx),
-             int(idx.dtype == torch.int64), n, k, _ptr(weight), ctypes.c_float(scale), _ptr(out))
+    _call_on(table, _L().ls3d_embedding_forward, "ls3d_embedding_forward", pt, ld, table.shape[0], c, DTYPES[table.dtype], _addr(idx),
+             int(idx.dtype == torch.int64), n, k, _addr(weight), scale, _addr(out))
     return out
 
 
@@ -1956,7 +1978,7 @@ def embedding_backward(table, idx, weight, scale, padding, dout, want_table=True
     dw = torch.empty((n, k), dtype=torch.float32, device=table.device) if want_weight else None
     L = _L()
     ws = _ws(L.ls3d_embedding_workspace_bytes(n, k, c), table)
-    (pt, ld), (po, o_ld), ll = _row_view(table, "table"), _row_view(dout, "dout"), ctypes.c_longlong
-    _call_on(table, L.ls3d_embedding_backward, "ls3d_embedding_backward", pt, ll(ld), ll(rows), c, DTYPES[table.dtype], _ptr(idx), int(idx.dtype == torch.int64), n, k,
-             _ptr(weight), ctypes.c_float(scale), ll(padding), po, ll(o_ld), _ptr(dt), _ptr(dw), _ptr(ws), ctypes.c_size_t(ws.numel()))
+    (pt, ld), (po, o_ld) = _row_view(table, "table"), _row_view(dout, "dout")
+    _call_on(table, L.ls3d_embedding_backward, "ls3d_embedding_backward", pt, ld, rows, c, DTYPES[table.dtype], _addr(idx), int(idx.dtype == torch.int64), n, k,
+             _addr(weight), scale, padding, po, o_ld, _addr(dt), _addr(dw), _addr(ws), ws.numel())
     return dt, dw
