@@ -13,6 +13,17 @@
 #else
 #define LS3D_OPAQUE(x) asm("" : "+v"(x))
 #endif
+
+// between an LDS access of some lanes and one of others of the same wave: the compiler keeps their order (the hardware does by itself)
+#ifdef HIPSIM
+#define LS3D_WAVE_SYNC() ((void)__ballot(1))
+#else
+#define LS3D_WAVE_SYNC()                               \
+  do {                                                 \
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); \
+    __builtin_amdgcn_wave_barrier();                   \
+  } while (0)
+#endif
 typedef __bf16 ls3d_bf16;
 typedef _Float16 ls3d_f16;
 typedef uint32_t ls3d_u32x4 __attribute__((ext_vector_type(4)));

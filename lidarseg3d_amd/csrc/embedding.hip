@@ -5,41 +5,51 @@
 //             dweight[i][k] = scale * <dout[i], table[idx[i][k]]>
 // An index outside [0, rows) names no row: it adds nothing and takes no gradient.  Sums in f32, rounded to the table's type once.
 //
-// The gradient: the entries are sorted by row (stable), cut into tiles of `tile` entries, and a group of lanes walks each tile, adding up dout rows as
-// long as the table row stays the same.  A row whose entries lie within one tile is written at once; one that crosses tiles leaves a partial sum
-// per tile, which k_emb_join adds in order.  So the work per group is the same whether every token is another one or all are the same, and the
-// order of the additions is fixed: no atomics, the same bits every time.  Rows without entries: the table's gradient is cleared first.
-// Bound by memory: n rows of dout in, the whole gradient table out.
+// The gradient: the entries that name a row are sorted by it (stable), cut into tiles of `tile` entries, and a group of lanes walks each tile, adding up
+// dout rows as long as the table row stays the same.  A row whose entries lie within one tile is written at once; one that crosses tiles leaves a
+// partial sum per tile, which k_emb_join adds in order.  So the work per group is the same whether every token is another one or all are the same, and
+// the order of the additions is fixed: no atomics on sums, the same bits every time.  Rows without entries: the table's gradient is cleared first.
+// Bound by memory: dout rows in, the whole gradient table out; the sort moves 8 bytes an entry and pass.
 #include "blocks_common.h"
-
-int ls3d_radix_sort_pairs(const uint32_t *keys_in, const int32_t *vals_in, int n, const int32_t *n_dev, int bits, uint32_t *keys_out, int32_t *vals_out,
-                          void *workspace, size_t workspace_bytes, hipStream_t stream);
 
 __device__ __forceinline__ long long emb_index(const void *__restrict__ idx, int is64, size_t e) {
   return is64 ? ((const long long *)idx)[e] : (long long)((const int32_t *)idx)[e];
 }
 
-// one chunk of 8 columns of one output row per thread and trip
-template <typename T>
-__global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, int n, int k,
+// one chunk of 8 columns of one output row per thread and trip; four indices, then four table rows in flight.  I: 32 bits where the chunk count allows
+template <typename T, typename I>
+__global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total, int k,
                                                  const float *__restrict__ weight, float scale, T *__restrict__ out) {
   const uint32_t groups = (uint32_t)(c + 7) / 8;
-  const long long total = (long long)n * groups;
-  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
-    const uint32_t i = (uint32_t)(t / groups), g = (uint32_t)(t - (long long)i * groups);
+  for (I t = (I)blockIdx.x * 256 + threadIdx.x; t < total; t += (I)gridDim.x * 256) {
+    const uint32_t i = (uint32_t)(t / groups), g = (uint32_t)(t - (I)i * groups);
     const int col = (int)g * 8, m = c - col;
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-    for (int q = 0; q < k; ++q) {
-      const size_t e = (size_t)i * k + q;
-      const long long v = emb_index(idx, is64, e);
-      if (v < 0 || v >= rows) continue;
-      const float w = weight ? weight[e] : 1.0f;
-      float r[8];
-      ls3d_unpack8<T>(ls3d_load8<T>(table + (size_t)v * table_ld, col, c), m, r);
+    for (int q0 = 0; q0 < k; q0 += 4) {
+      long long v[4];
+      float w[4];
+      ls3d_raw8<T> r[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = weight ? fmaf(w, r[j], acc[j]) : acc[j] + r[j];
+      for (int q = 0; q < 4; ++q) {
+        const size_t e = (size_t)i * k + (q0 + q < k ? q0 + q : k - 1);
+        v[q] = q0 + q < k ? emb_index(idx, is64, e) : -1;
+        w[q] = weight ? weight[e] : 1.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        r[q] = ls3d_raw8<T>{};
+        if (v[q] >= 0 && v[q] < rows) r[q] = ls3d_load8<T>(table + (size_t)v[q] * table_ld, col, c);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (v[q] < 0 || v[q] >= rows) continue;
+        float x[8];
+        ls3d_unpack8<T>(r[q], m, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = fmaf(w[q], x[j], acc[j]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] *= scale;
@@ -47,61 +57,289 @@ __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, si
   }
 }
 
-// sort keys (the table row; `rows` for an entry without one) and the cleared gradient
+// ---- the entries sorted by table row: pairs (row, entry), stable, the entries without a row left out; *n_valid = how many there are.
+//      LSD radix passes of up to 11 bits (a table of up to 4 M rows: two), the first one straight from the indices.
+constexpr int ES_ITEMS = 16;              // entries a thread
+constexpr int ES_TILE = 256 * ES_ITEMS;   // entries a workgroup
+constexpr int ES_MAX_DIGITS = 2048;
+
+struct emb_keys { const void *idx; int is64; long long rows, padding; };  // where an entry's row comes from in the first pass
+__device__ __forceinline__ uint32_t emb_key(const emb_keys &K, size_t e) {  // 0xFFFFFFFF: no row
+  const long long v = emb_index(K.idx, K.is64, e);
+  return v < 0 || v >= K.rows || v == K.padding ? 0xFFFFFFFFu : (uint32_t)v;
+}
+
+// clears the gradient table, a share per workgroup (rides along with the launches that only read the indices)
 template <typename T>
-__global__ __launch_bounds__(256) void k_emb_keys(const void *__restrict__ idx, int is64, int entries, long long rows, long long padding, uint32_t *__restrict__ keys,
-                                                  T *__restrict__ dtable, size_t elems) {
-  const size_t t0 = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
-  for (size_t e = t0; e < (size_t)entries; e += step) {
-    const long long v = emb_index(idx, is64, e);
-    keys[e] = (uint32_t)(v < 0 || v >= rows || v == padding ? rows : v);
-  }
+__device__ __forceinline__ void emb_clear(T *__restrict__ dtable, size_t elems, size_t t0, size_t step) {
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (size_t g = t0; g * 8 < elems; g += step) ls3d_store8<T>(dtable + g * 8, zero, elems - g * 8 < 8 ? (int)(elems - g * 8) : 8);
 }
 
-// grid (groups of tiles, column slabs): `lpr` lanes per tile, a chunk of 8 columns each
+// per-workgroup digit counts -> hist[workgroup][digit]; FIRST: from the indices, and the gradient table is cleared by the same launch
+template <typename T, bool FIRST>
+__global__ __launch_bounds__(256) void k_es_hist(emb_keys K, const uint2 *__restrict__ pairs, int entries, const int32_t *__restrict__ n_valid, int shift, int digits, int ntiles,
+                                                 int32_t *__restrict__ hist, T *__restrict__ dtable, size_t elems) {
+  __shared__ int s_h[ES_MAX_DIGITS];
+  if ((int)blockIdx.x < ntiles) {
+    const int N = FIRST ? entries : *n_valid;
+    const long long lo = (long long)blockIdx.x * ES_TILE;
+    for (int d = threadIdx.x; d < digits; d += 256) s_h[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ES_ITEMS; ++i) {
+      const long long e = lo + i * 256 + threadIdx.x;
+      if (e < N) {
+        const uint32_t key = FIRST ? emb_key(K, (size_t)e) : pairs[e].x;
+        if (!FIRST || key != 0xFFFFFFFFu) atomicAdd(&s_h[(key >> shift) & (digits - 1)], 1);
+      }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += 256) hist[(size_t)blockIdx.x * digits + d] = s_h[d];
+  }
+  if (FIRST) emb_clear<T>(dtable, elems, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
+}
+
+// hist[workgroup][digit] -> the digit's count in the workgroups before, totals[digit]: 64 digits x 16 segments of workgroups per workgroup
+__global__ __launch_bounds__(1024) void k_es_scan(int32_t *__restrict__ hist, int ntiles, int digits, int32_t *__restrict__ totals) {
+  __shared__ int s_seg[16][64];
+  const int d = blockIdx.x * 64 + (threadIdx.x & 63), seg = threadIdx.x >> 6, per = (ntiles + 15) / 16;
+  const int lo = seg * per, hi = lo + per < ntiles ? lo + per : ntiles;
+  const bool on = d < digits;
+  int s = 0;
+  for (int b = lo; b < hi; b += 8) {
+    int v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s += v[q];
+  }
+  s_seg[seg][threadIdx.x & 63] = s;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int x = s_seg[q][threadIdx.x & 63];
+    before += q < seg ? x : 0;
+    total += x;
+  }
+  for (int b = lo; b < hi; b += 8) {
+    int v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (on && b + q < hi) { hist[(size_t)(b + q) * digits + d] = before; before += v[q]; }
+  }
+  if (on && seg == 0) totals[d] = total;
+}
+
+// lanes of the wave that hold a live item with this lane's digit
+__device__ __forceinline__ unsigned long long emb_peers(bool live, uint32_t d, int bits) {
+  unsigned long long peers = __ballot(live);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned long long m = __ballot((d >> b) & 1u);
+    peers &= ((d >> b) & 1u) ? m : ~m;
+  }
+  return peers;
+}
+
+// exclusive sums of v over the workgroup's 64 * W threads, in thread order; *total: their sum (s_w: W ints)
+template <int W>
+__device__ __forceinline__ int emb_block_scan(int v, int *s_w, int *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(s, d);
+    s += lane >= d ? u : 0;
+  }
+  if (lane == 63) s_w[wave] = s;
+  __syncthreads();
+  int before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    before += w < wave ? s_w[w] : 0;
+    sum += s_w[w];
+  }
+  *total = sum;
+  return before + s - v;
+}
+
+// places a tile's items: a wave takes 64 * ES_ITEMS consecutive ones, 64 at a time; an item's rank among its wave's equal digits from ballots and a count per
+// wave and digit, the waves' and workgroups' shares on top.  Equal digits keep their order.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void k_es_scatter(emb_keys K, const uint2 *__restrict__ pairs, int entries, int32_t *__restrict__ n_valid, int shift, int digits, int bits,
+                                                    const int32_t *__restrict__ hist, const int32_t *__restrict__ totals, uint2 *__restrict__ out) {
+  __shared__ int s_cnt[4][ES_MAX_DIGITS];
+  __shared__ int s_w[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int N = FIRST ? entries : *n_valid;
+  const long long lo = (long long)blockIdx.x * ES_TILE;
+  if (lo >= N) return;  // (the first pass: every workgroup has items)
+  for (int d = threadIdx.x; d < digits; d += 256) s_cnt[0][d] = s_cnt[1][d] = s_cnt[2][d] = s_cnt[3][d] = 0;
+  uint2 item[ES_ITEMS];
+  int rank[ES_ITEMS];
+#pragma unroll
+  for (int i = 0; i < ES_ITEMS; ++i) {
+    const long long e = lo + (wave * ES_ITEMS + i) * 64 + lane;
+    item[i].x = 0xFFFFFFFFu;
+    item[i].y = (unsigned)e;
+    if (e < N) {
+      if (FIRST) item[i].x = emb_key(K, (size_t)e);
+      else item[i] = pairs[e];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ES_ITEMS; ++i) {
+    const bool live = item[i].x != 0xFFFFFFFFu;
+    const uint32_t d = (item[i].x >> shift) & (uint32_t)(digits - 1);
+    const unsigned long long peers = emb_peers(live, d, bits);
+    const int before = __popcll(peers & ((1ull << lane) - 1ull));
+    rank[i] = before + (live ? s_cnt[wave][d] : 0);
+    LS3D_WAVE_SYNC();
+    if (live && before == 0) s_cnt[wave][d] += __popcll(peers);
+    LS3D_WAVE_SYNC();
+  }
+  __syncthreads();
+  // where each digit starts: the digits below in all workgroups, the digit itself in the workgroups and waves before
+  const int per = (digits + 255) / 256, d0 = (int)threadIdx.x * per;
+  int mine = 0, total;
+  for (int q = 0; q < per; ++q) mine += d0 + q < digits ? totals[d0 + q] : 0;
+  int base = emb_block_scan<4>(mine, s_w, &total);
+  for (int q = 0; q < per; ++q) {
+    const int d = d0 + q;
+    if (d >= digits) break;
+    int s = base + hist[(size_t)blockIdx.x * digits + d];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int x = s_cnt[w][d];
+      s_cnt[w][d] = s;
+      s += x;
+    }
+    base += totals[d];
+  }
+  if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *n_valid = total;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ES_ITEMS; ++i)
+    if (item[i].x != 0xFFFFFFFFu) out[s_cnt[wave][(item[i].x >> shift) & (uint32_t)(digits - 1)] + rank[i]] = item[i];
+}
+
+// few entries (<= 1024 * ITEMS): workgroup 0 sorts them all in LDS, 8 bits a pass, while the others clear the gradient table - one launch
+template <typename T, int ITEMS>
+__global__ __launch_bounds__(1024) void k_es_small(emb_keys K, int entries, int bits, int32_t *__restrict__ n_valid, uint2 *__restrict__ out, T *__restrict__ dtable, size_t elems) {
+  HIP_DYNAMIC_SHARED(char, smem)
+  uint2 *s_item = (uint2 *)smem;                                    // [1024 * ITEMS]
+  int (*s_cnt)[256] = (int (*)[256])(smem + 1024 * ITEMS * sizeof(uint2));  // [16 waves][256 digits]
+  __shared__ int s_w[16];
+  if (blockIdx.x > 0 || gridDim.x == 1) {
+    const size_t first = gridDim.x == 1 ? 0 : blockIdx.x - 1, others = gridDim.x == 1 ? 1 : gridDim.x - 1;
+    emb_clear<T>(dtable, elems, first * 1024 + threadIdx.x, others * 1024);
+    if (blockIdx.x > 0) return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint2 item[ITEMS];
+  int rank[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int e = (wave * ITEMS + i) * 64 + lane;
+    item[i].x = e < entries ? emb_key(K, (size_t)e) : 0xFFFFFFFFu;
+    item[i].y = (unsigned)e;
+  }
+  int total = 0;
+  for (int shift = 0; shift < bits; shift += 8) {
+    for (int d = threadIdx.x; d < 16 * 256; d += 1024) s_cnt[d >> 8][d & 255] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool live = item[i].x != 0xFFFFFFFFu;
+      const uint32_t d = (item[i].x >> shift) & 255u;
+      const unsigned long long peers = emb_peers(live, d, 8);
+      const int before = __popcll(peers & ((1ull << lane) - 1ull));
+      rank[i] = before + (live ? s_cnt[wave][d] : 0);
+      LS3D_WAVE_SYNC();
+      if (live && before == 0) s_cnt[wave][d] += __popcll(peers);
+      LS3D_WAVE_SYNC();
+    }
+    __syncthreads();
+    int mine = 0;
+    if (threadIdx.x < 256)
+      for (int w = 0; w < 16; ++w) mine += s_cnt[w][threadIdx.x];
+    int s = emb_block_scan<16>(mine, s_w, &total);
+    if (threadIdx.x < 256)
+      for (int w = 0; w < 16; ++w) {
+        const int x = s_cnt[w][threadIdx.x];
+        s_cnt[w][threadIdx.x] = s;
+        s += x;
+      }
+    __syncthreads();
+    uint2 *dst = shift + 8 >= bits ? out : s_item;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (item[i].x != 0xFFFFFFFFu) dst[s_cnt[wave][(item[i].x >> shift) & 255u] + rank[i]] = item[i];
+    if (shift + 8 >= bits) break;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int e = (wave * ITEMS + i) * 64 + lane;
+      item[i].x = 0xFFFFFFFFu;
+      if (e < total) item[i] = s_item[e];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *n_valid = total;
+}
+
+// grid (groups of tiles, column slabs): `lpr` lanes per tile, a chunk of 8 columns each; four entries' rows in flight
 template <typename T>
-__global__ __launch_bounds__(256) void k_emb_tiles(const uint32_t *__restrict__ keys, const int32_t *__restrict__ order, int entries, int tile, int lpr, long long rows, int c,
-                                                   int k, const float *__restrict__ weight, float scale, const T *__restrict__ dout, size_t dout_ld,
+__global__ __launch_bounds__(256) void k_emb_tiles(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int lpr, int c, int k,
+                                                   const float *__restrict__ weight, float scale, const T *__restrict__ dout, size_t dout_ld,
                                                    T *__restrict__ dtable, float *__restrict__ partial) {
-  const int lane = threadIdx.x % lpr, per = 256 / lpr;
-  const long long j = (long long)blockIdx.x * per + threadIdx.x / lpr;
-  const long long lo = j * tile;
+  const int lane = threadIdx.x % lpr, per = 256 / lpr, N = *n_valid;
+  const long long j = (long long)blockIdx.x * per + threadIdx.x / lpr, lo = j * tile;
   const int col = ((int)blockIdx.y * lpr + lane) * 8, m = c - col;
-  if (lo >= entries || m <= 0) return;
-  const int hi = lo + tile < entries ? (int)(lo + tile) : entries;
-  uint32_t cur = keys[lo];
-  bool from_before = lo > 0 && keys[lo - 1] == cur;  // the open row began in an earlier tile
+  if (lo >= N || m <= 0) return;
+  const int hi = lo + tile < N ? (int)(lo + tile) : N;
+  uint32_t cur = pairs[lo].x;
+  bool from_before = lo > 0 && pairs[lo - 1].x == cur;  // the open row began in an earlier tile
+  const bool goes_on = hi < N && pairs[hi < N ? hi : 0].x == pairs[hi - 1].x;
   float acc[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
-  for (int e = (int)lo; e < hi; ++e) {
-    const uint32_t key = keys[e];
-    if (key != cur) {
-      if (cur < (uint32_t)rows) {
+  for (int e0 = (int)lo; e0 < hi; e0 += 4) {
+    uint2 pr[4];
+    float w[4];
+    ls3d_raw8<T> r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) pr[u] = pairs[e0 + u < hi ? e0 + u : hi - 1];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      w[u] = weight ? weight[pr[u].y] : 1.0f;
+      r[u] = ls3d_load8<T>(dout + (size_t)(k == 1 ? pr[u].y : pr[u].y / (unsigned)k) * dout_ld, col, c);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (e0 + u >= hi) continue;
+      if (pr[u].x != cur) {  // the same for every lane of the group
         if (from_before) ls3d_store8<float>(partial + ((size_t)j * 2) * c + col, acc, m);
         else {
 #pragma unroll
           for (int q = 0; q < 8; ++q) acc[q] *= scale;
           ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
         }
+        cur = pr[u].x;
+        from_before = false;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
       }
-      cur = key;
-      from_before = false;
+      float g[8];
+      ls3d_unpack8<T>(r[u], m, g);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
+      for (int q = 0; q < 8; ++q) acc[q] = fmaf(w[u], g[q], acc[q]);
     }
-    if (key >= (uint32_t)rows) break;  // sorted: entries without a row come last
-    const int ent = order[e];
-    float g[8];
-    ls3d_unpack8<T>(ls3d_load8<T>(dout + (size_t)(k == 1 ? ent : ent / k) * dout_ld, col, c), m, g);
-    const float w = weight ? weight[ent] : 1.0f;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] = fmaf(w, g[q], acc[q]);
   }
-  if (cur >= (uint32_t)rows) return;
-  const bool goes_on = hi < entries && keys[hi] == cur;
   if (from_before) ls3d_store8<float>(partial + ((size_t)j * 2) * c + col, acc, m);
   else if (goes_on) ls3d_store8<float>(partial + ((size_t)j * 2 + 1) * c + col, acc, m);
   else {
@@ -115,18 +353,20 @@ __global__ __launch_bounds__(256) void k_emb_tiles(const uint32_t *__restrict__ 
 // `lpr` lanes per partial row, the 256 / lpr groups take the tiles in turn (one wave walking the 700 tiles of a row one after the other took 210 us), their
 // sums are added in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_emb_join(const uint32_t *__restrict__ keys, int entries, int tile, int ntiles, int lpr, long long rows, int c, float scale,
+__global__ __launch_bounds__(256) void k_emb_join(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int lpr, int c, float scale,
                                                   const float *__restrict__ partial, T *__restrict__ dtable) {
   __shared__ float s_sum[256][9];
-  const int j = (int)blockIdx.x;
+  const int j = (int)blockIdx.x, N = *n_valid;
   const long long hi = (long long)(j + 1) * tile;
-  const uint32_t cur = keys[hi - 1];
-  if (cur >= (uint32_t)rows || keys[hi] != cur) return;  // nothing goes on (uniform over the workgroup, like the next line)
-  if (j > 0 && keys[hi - tile] == cur && keys[hi - tile - 1] == cur) return;  // it began in an earlier tile
-  int last = j + 1;  // the last tile that begins with this row: sorted keys, so those that do are the first of any run of tiles
+  if (hi >= N) return;
+  const int ntiles = (int)(((long long)N + tile - 1) / tile);
+  const uint32_t cur = pairs[hi - 1].x;
+  if (pairs[hi].x != cur) return;  // nothing goes on (uniform over the workgroup, like the next line)
+  if (j > 0 && pairs[hi - tile].x == cur && pairs[hi - tile - 1].x == cur) return;  // it began in an earlier tile
+  int last = j + 1;  // the last tile that begins with this row: sorted, so those that do are the first of any run of tiles
   for (;;) {
     const long long t = (long long)last + 1 + threadIdx.x;
-    const int on = __syncthreads_count(t < ntiles && keys[t < ntiles ? t * tile : 0] == cur);
+    const int on = __syncthreads_count(t < ntiles && pairs[t < ntiles ? t * tile : 0].x == cur);
     last += on;
     if (on < 256) break;
   }
@@ -158,27 +398,28 @@ __global__ __launch_bounds__(256) void k_emb_join(const uint32_t *__restrict__ k
   }
 }
 
-// dweight: a wave per output row, its dout row read once per 512 columns and entry
+// dweight: `lpr` lanes per entry
 template <typename T>
-__global__ __launch_bounds__(256) void k_emb_dweight(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, int n, int k,
-                                                     float scale, const T *__restrict__ dout, size_t dout_ld, float *__restrict__ dweight) {
-  const int lane = threadIdx.x & 63;
-  for (long long e = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); e < (long long)n * k; e += (long long)gridDim.x * 4) {
-    const long long v = emb_index(idx, is64, (size_t)e);
+__global__ __launch_bounds__(256) void k_emb_dweight(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, long long entries,
+                                                     int k, int lpr, float scale, const T *__restrict__ dout, size_t dout_ld, float *__restrict__ dweight) {
+  const int lane = threadIdx.x % lpr, per = 256 / lpr;
+  for (long long e0 = (long long)blockIdx.x * per; e0 < entries; e0 += (long long)gridDim.x * per) {  // the same trips for every lane of a wave
+    const long long e = e0 + threadIdx.x / lpr;
+    const long long v = e < entries ? emb_index(idx, is64, (size_t)e) : -1;
     float s = 0.0f;
     if (v >= 0 && v < rows) {
       const size_t i = (size_t)(e / k);
-      for (int col = lane * 8; col < c; col += 512) {
+      for (int col = lane * 8; col < c; col += lpr * 8) {
         float a[8], b[8];
-        ls3d_unpack8<T>(ls3d_load8<T>(table + (size_t)v * table_ld, col, c), c - col, a);
-        ls3d_unpack8<T>(ls3d_load8<T>(dout + i * dout_ld, col, c), c - col, b);
+        const ls3d_raw8<T> ra = ls3d_load8<T>(table + (size_t)v * table_ld, col, c), rb = ls3d_load8<T>(dout + i * dout_ld, col, c);
+        ls3d_unpack8<T>(ra, c - col, a);
+        ls3d_unpack8<T>(rb, c - col, b);
 #pragma unroll
         for (int q = 0; q < 8; ++q) s = fmaf(a[q], b[q], s);
       }
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) dweight[e] = s * scale;
+    for (int d = lpr >> 1; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+    if (lane == 0 && e < entries) dweight[e] = s * scale;
   }
 }
 
@@ -204,9 +445,15 @@ extern "C" int ls3d_embedding_forward(const void *table, long long table_ld, lon
   const int rc = emb_check(table, table_ld, rows, c, dtype, idx, idx_dtype, n, k, weight);
   if (rc != LS3D_OK || n == 0 || c == 0) return rc;
   if (!out || ((uintptr_t)out & (ls3d_dtype_size(dtype) - 1))) return LS3D_ERR_ARG;
-  const dim3 grid = ls3d_grid((long long)n * ((c + 7) / 8));
-  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T>), grid, dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, (int)(idx_dtype == LS3D_INDEX_I64), n, k,
-                                      weight, scale, (T *)out));
+  const long long total = (long long)n * ((c + 7) / 8);
+  const int is64 = idx_dtype == LS3D_INDEX_I64;
+  const dim3 grid = ls3d_grid(total);
+  if (total < (1ll << 31))
+    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, uint32_t>), grid, dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (uint32_t)total, k, weight,
+                                        scale, (T *)out));
+  else
+    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, unsigned long long>), grid, dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,
+                                        (unsigned long long)total, k, weight, scale, (T *)out));
   LS3D_RETURN_IF_LAUNCH_FAILED();
   return LS3D_OK;
 }
@@ -219,12 +466,99 @@ static inline int emb_tile(long long entries, int c) {
   return t;
 }
 
+// the sorting of a call: up to ES_SMALL entries in one workgroup, else radix passes of at most 11 bits, as even as they come
+constexpr int ES_SMALL = 16384;
+static inline int emb_passes(int bits) { return (bits + 10) / 11; }
+
+struct emb_space { size_t pairs[2], partial, hist, totals, n_valid, bytes; };  // byte offsets in the workspace
+static emb_space emb_layout(long long entries, int c) {
+  emb_space s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t p = at; at += (bytes + 255) / 256 * 256; return p; };
+  const int tile = emb_tile(entries, c);
+  s.n_valid = take(4);
+  s.totals = take(ES_MAX_DIGITS * 4);
+  s.pairs[0] = take((size_t)entries * 8);
+  s.pairs[1] = take(entries > ES_SMALL ? (size_t)entries * 8 : 0);
+  s.hist = take(entries > ES_SMALL ? (size_t)((entries + ES_TILE - 1) / ES_TILE) * ES_MAX_DIGITS * 4 : 0);
+  s.partial = take((size_t)((entries + tile - 1) / tile) * 2 * c * sizeof(float));
+  s.bytes = at + 256;
+  return s;
+}
+
 extern "C" size_t ls3d_embedding_workspace_bytes(int n, int k, int c) {
   if (n < 0 || k < 1 || c < 0 || (long long)n * k > 0x3FFFFFFFll) return 0;
-  const long long e = (long long)n * k;
-  const int tile = emb_tile(e, c);
-  const size_t part = (size_t)((e + tile - 1) / tile) * 2 * c * sizeof(float);
-  return ((size_t)e * 4 + 255) / 256 * 256 * 3 + (part + 255) / 256 * 256 + ls3d_radix_sort_workspace_bytes((int)e) + 256;
+  return emb_layout((long long)n * k, c).bytes;
+}
+
+template <typename T, int ITEMS>
+static bool emb_sort_small(const emb_keys &K, int entries, int bits, int32_t *n_valid, uint2 *out, T *dtable, size_t elems, hipStream_t stream) {
+  const int lds = 1024 * ITEMS * (int)sizeof(uint2) + 16 * 256 * 4;
+  static bool attr_set[LS3D_MAX_DEVICES] = {};  // the opt-in to > 64 KB of dynamic LDS is per device
+  bool &set = attr_set[ls3d_device_slot()];
+  if (!set && lds > 65536) {
+    if (hipFuncSetAttribute((const void *)k_es_small<T, ITEMS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return false;
+    set = true;
+  }
+  hipLaunchKernelGGL((k_es_small<T, ITEMS>), dim3(1 + ls3d_grid((long long)(elems / 8 + 1), 1024, 1024).x), dim3(1024), lds, stream, K, entries, bits, n_valid, out, dtable, elems);
+  return true;
+}
+
+// sorts the entries and clears the gradient table; -> the sorted pairs
+template <typename T>
+static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S, char *ws, T *dtable, size_t elems, hipStream_t stream) {
+  int bits = 1;
+  while (((K.rows - 1) >> bits) != 0) ++bits;
+  int32_t *n_valid = (int32_t *)(ws + S.n_valid), *totals = (int32_t *)(ws + S.totals), *hist = (int32_t *)(ws + S.hist);
+  uint2 *buf[2] = {(uint2 *)(ws + S.pairs[0]), (uint2 *)(ws + S.pairs[1])};
+  if (entries <= ES_SMALL) {
+    const bool ok = entries <= 1024   ? emb_sort_small<T, 1>(K, entries, bits, n_valid, buf[0], dtable, elems, stream)
+                    : entries <= 4096 ? emb_sort_small<T, 4>(K, entries, bits, n_valid, buf[0], dtable, elems, stream)
+                                      : emb_sort_small<T, 16>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
+    return ok ? buf[0] : nullptr;
+  }
+  const int passes = emb_passes(bits), per = (bits + passes - 1) / passes, ntiles = (entries + ES_TILE - 1) / ES_TILE, digits = 1 << per;
+  const unsigned clear = ls3d_grid((long long)(elems / 8 + 1)).x;
+  for (int p = 0; p < passes; ++p) {
+    uint2 *out = buf[p & 1], *in = buf[1 - (p & 1)];
+    if (p == 0) {
+      hipLaunchKernelGGL((k_es_hist<T, true>), dim3((unsigned)ntiles > clear ? (unsigned)ntiles : clear), dim3(256), 0, stream, K, (const uint2 *)nullptr, entries,
+                         (const int32_t *)nullptr, 0, digits, ntiles, hist, dtable, elems);
+    } else {
+      hipLaunchKernelGGL((k_es_hist<T, false>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, (const int32_t *)n_valid, p * per, digits, ntiles,
+                         hist, dtable, elems);
+    }
+    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 63) / 64)), dim3(1024), 0, stream, hist, ntiles, digits, totals);
+    if (p == 0)
+      hipLaunchKernelGGL((k_es_scatter<true>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)nullptr, entries, n_valid, 0, digits, per, (const int32_t *)hist,
+                         (const int32_t *)totals, out);
+    else
+      hipLaunchKernelGGL((k_es_scatter<false>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, n_valid, p * per, digits, per, (const int32_t *)hist,
+                         (const int32_t *)totals, out);
+  }
+  return buf[(passes - 1) & 1];
+}
+
+template <typename T>
+static int emb_table_gradient(const emb_keys &K, int entries, int c, int k, const float *weight, float scale, const T *dout, size_t dout_ld, T *dtable, char *ws, hipStream_t stream) {
+  const size_t elems = (size_t)K.rows * c;
+  const emb_space S = emb_layout(entries, c);
+  const uint2 *pairs = emb_sort<T>(K, entries, S, ws, dtable, elems, stream);
+  if (!pairs) return LS3D_ERR_LAUNCH;
+  const int groups = (c + 7) / 8, tile = emb_tile(entries, c), ntiles = (entries + tile - 1) / tile;
+  int lpr = 1;
+  while (lpr < groups && lpr < 64) lpr *= 2;
+  const dim3 grid((unsigned)((ntiles + 256 / lpr - 1) / (256 / lpr)), (unsigned)((groups + lpr - 1) / lpr));
+  const int32_t *n_valid = (const int32_t *)(ws + S.n_valid);
+  float *partial = (float *)(ws + S.partial);
+  hipLaunchKernelGGL((k_emb_tiles<T>), grid, dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, k, weight, scale, dout, dout_ld, dtable, partial);
+  if (ntiles > 1) hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)(ntiles - 1), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, scale, (const float *)partial, dtable);
+  return LS3D_OK;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_emb_clear(T *__restrict__ dtable, size_t elems) {
+  emb_clear<T>(dtable, elems, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
 
 extern "C" int ls3d_embedding_backward(const void *table, long long table_ld, long long rows, int c, int dtype, const void *idx, int idx_dtype, int n, int k,
@@ -236,36 +570,25 @@ extern "C" int ls3d_embedding_backward(const void *table, long long table_ld, lo
   if (rc != LS3D_OK) return rc;
   const size_t elem = ls3d_dtype_size(dtype);
   if ((n > 0 && c > 0 && (!dout || dout_ld < c || ((uintptr_t)dout & (elem - 1)))) || ((uintptr_t)dtable & (elem - 1)) || ((uintptr_t)dweight & 3)) return LS3D_ERR_ARG;
-  const int is64 = idx_dtype == LS3D_INDEX_I64, entries = n * k, groups = (c + 7) / 8;
-  if (dweight && entries > 0 && c > 0)
-    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_dweight<T>), ls3d_grid(entries, 4), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, n, k, scale,
-                                        (const T *)dout, (size_t)dout_ld, dweight));
+  const int is64 = idx_dtype == LS3D_INDEX_I64, entries = n * k;
+  if (dtable && rows > 0 && c > 0 && entries > 0) {
+    if (!workspace || ((uintptr_t)workspace & 15)) return LS3D_ERR_ARG;
+    if (workspace_bytes < ls3d_embedding_workspace_bytes(n, k, c)) return LS3D_ERR_WORKSPACE;
+  }
+  if (dweight && entries > 0 && c > 0) {
+    int lpr = 1;
+    while (lpr * 8 < c && lpr < 64) lpr *= 2;
+    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_dweight<T>), ls3d_grid(entries, 256 / lpr), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,
+                                        (long long)entries, k, lpr, scale, (const T *)dout, (size_t)dout_ld, dweight));
+  }
   if (dtable && rows > 0 && c > 0) {
-    if (entries > 0 && (!workspace || ((uintptr_t)workspace & 15))) return LS3D_ERR_ARG;
-    if (entries > 0 && workspace_bytes < ls3d_embedding_workspace_bytes(n, k, c)) return LS3D_ERR_WORKSPACE;
-    const size_t seg = ((size_t)entries * 4 + 255) / 256 * 256;
-    uint32_t *keys = (uint32_t *)workspace, *skeys = (uint32_t *)((char *)workspace + seg);
-    int32_t *order = (int32_t *)((char *)workspace + 2 * seg);
-    const int tile = emb_tile(entries, c), ntiles = (entries + tile - 1) / tile;
-    float *partial = (float *)((char *)workspace + 3 * seg);
-    const size_t part = ((size_t)ntiles * 2 * c * sizeof(float) + 255) / 256 * 256;
-    void *sort_ws = (char *)workspace + 3 * seg + part;
-    const size_t elems = (size_t)rows * c;
-    const long long work = (long long)(elems / 8 + 1) > entries ? (long long)(elems / 8 + 1) : entries;
-    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_keys<T>), ls3d_grid(work), dim3(256), 0, stream, idx, is64, entries, rows, padding, keys, (T *)dtable, elems));
+    const emb_keys K = {idx, is64, rows, padding};
     if (entries > 0) {
-      int bits = 1;
-      while ((rows >> bits) != 0) ++bits;  // keys 0 .. rows
-      rc = ls3d_radix_sort_pairs(keys, nullptr, entries, nullptr, bits, skeys, order, sort_ws, ls3d_radix_sort_workspace_bytes(entries), stream);
+      EMB_TYPES(dtype, rc = emb_table_gradient<T>(K, entries, c, k, weight, scale, (const T *)dout, (size_t)dout_ld, (T *)dtable, (char *)workspace, stream));
       if (rc != LS3D_OK) return rc;
-      int lpr = 1;
-      while (lpr < groups && lpr < 64) lpr *= 2;
-      const dim3 grid((unsigned)((ntiles + 256 / lpr - 1) / (256 / lpr)), (unsigned)((groups + lpr - 1) / lpr));
-      EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_tiles<T>), grid, dim3(256), 0, stream, (const uint32_t *)skeys, (const int32_t *)order, entries, tile, lpr, rows, c, k, weight,
-                                          scale, (const T *)dout, (size_t)dout_ld, (T *)dtable, partial));
-      if (ntiles > 1)
-        EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)(ntiles - 1), grid.y), dim3(256), 0, stream, (const uint32_t *)skeys, entries, tile,
-                                            ntiles, lpr, rows, c, scale, (const float *)partial, (T *)dtable));
+    } else {
+      const size_t elems = (size_t)rows * c;
+      EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_clear<T>), ls3d_grid((long long)(elems / 8 + 1)), dim3(256), 0, stream, (T *)dtable, elems));
     }
   }
   LS3D_RETURN_IF_LAUNCH_FAILED();

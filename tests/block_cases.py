@@ -197,6 +197,11 @@ EMBEDDING = [
     (70000, 5, F32, (90,), False, False, 1.0, "uniform"),
     (12, 1030, BF16, (70,), False, False, 32.0, "few"),
     (9, 64, F32, (1300,), False, False, 1.0, "one"),
+    (2500, 3, F32, (5000,), False, False, 1.0, "uniform"),
+    # more entries than one workgroup sorts: radix passes of one digit, of two, with entries that name no row
+    (300, 2, F32, (16500,), False, False, 1.0, "uniform"),
+    (9000, 3, F16, (17001,), False, False, 1.0, "uniform"),
+    (70, 4, F32, (6000, 3), True, True, 1.0, "holes"),
 ]
 
 

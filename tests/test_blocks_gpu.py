@@ -26,6 +26,8 @@ def test_residual_norm(case):
 @pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
 @pytest.mark.parametrize("case", bc.EMBEDDING + [
     (32, 64, bc.F32, (40000,), False, False, 1.0, "uniform"),
+    (5000000, 2, bc.F32, (20000,), False, False, 1.0, "uniform"),
+    (30000, 16, bc.BF16, (300000,), False, False, 1.0, "uniform"),
     (3, 64, bc.BF16, (30011,), False, False, 1.0, "few"),
     (20000, 48, bc.F32, (9000, 8), True, True, 1.0, "holes"),
     (2, 1024, bc.F16, (5003,), False, False, 1.0, "one"),
