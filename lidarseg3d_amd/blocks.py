@@ -83,6 +83,8 @@ def _on_device(t, what):
 def _rows(t, c):
     """t [..., c] as rows the kernels take: a view where the rows are contiguous, else a copy"""
     r = t if t.dim() == 2 else t.reshape(-1, c) if c else t.reshape(0, 0)
+    if r.is_contiguous():
+        return r
     if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < c):
         r = r.contiguous()
     return r
@@ -190,6 +192,25 @@ class _ResidualNorm(torch.autograd.Function):
         return (*out, None, None)
 
 
+def _norm_arguments(nm, c, what):
+    """-> weight, bias, kind, eps of a Norm or None, checked against rows of c values"""
+    if nm is None:
+        return None, None, 0, 0.0
+    if not isinstance(nm, Norm):
+        raise TypeError("%s: a blocks.Norm needed, got %s" % (what, type(nm).__name__))
+    out = []
+    for t in (nm.weight, nm.bias):
+        if t is not None:
+            if t.dtype not in ops.DTYPES:
+                _dtype_ok(t, what + " parameter")
+            if t.dim() != 1 or t.shape[0] != c:
+                raise ValueError("%s: weight and bias of shape [%d] needed, got %s" % (what, c, tuple(t.shape)))
+            if not t.is_contiguous():
+                t = t.contiguous()
+        out.append(t)
+    return out[0], out[1], _KINDS[nm.kind], nm.eps
+
+
 def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.0, p=0.0, state=None, call=None, return_sum=False):
     """One pass over a block's output x [..., c] and the residual stream:
 
@@ -216,29 +237,21 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
                 raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
             gate = _rows(gate, c)
         elif gate.numel() == 1 or gate.shape == (c,):
-            gate = (gate if gate.shape == (c,) else gate.reshape(1).expand(c)).contiguous()
+            gate = gate if gate.shape == (c,) else gate.reshape(1).expand(c)
+            if not gate.is_contiguous():
+                gate = gate.contiguous()
         else:
             raise ValueError("gate %s: one value, [%d] or %s" % (tuple(gate.shape), c, tuple(shape)))
-    params = []
-    for nm, what in ((norm_in, "norm_in"), (norm, "norm")):
-        if nm is not None and not isinstance(nm, Norm):
-            raise TypeError("%s: a blocks.Norm needed, got %s" % (what, type(nm).__name__))
-        for t, part in ((nm.weight, "weight"), (nm.bias, "bias")) if nm is not None else ((None, ""), (None, "")):
-            if t is not None:
-                _dtype_ok(t, "%s.%s" % (what, part))
-                if t.shape != (c,):
-                    raise ValueError("%s.%s %s: [%d] needed" % (what, part, tuple(t.shape), c))
-                t = t.contiguous()
-            params.append(t)
+    w_in, b_in, kind_in, eps_in = _norm_arguments(norm_in, c, "norm_in")
+    w_out, b_out, kind_out, eps_out = _norm_arguments(norm, c, "norm")
     p, state, call = _draw(p, state, call)
     x2, r2 = _rows(x, c), None if residual is None else _rows(residual, c)
-    kind_in, kind_out = _KINDS[norm_in.kind] if norm_in is not None else 0, _KINDS[norm.kind] if norm is not None else 0
-    eps_in, eps_out = norm_in.eps if norm_in is not None else 0.0, norm.eps if norm is not None else 0.0
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in [x2, r2, gate] + params):
-        res = _ResidualNorm.apply(x2, r2, gate, *params, state, (kind_in, eps_in, kind_out, eps_out, float(alpha), p, call, bool(return_sum)))
+    alpha, return_sum = float(alpha), bool(return_sum)
+    if torch.is_grad_enabled() and (x2.requires_grad or any(t is not None and t.requires_grad for t in (r2, gate, w_in, b_in, w_out, b_out))):
+        res = _ResidualNorm.apply(x2, r2, gate, w_in, b_in, w_out, b_out, state, (kind_in, eps_in, kind_out, eps_out, alpha, p, call, return_sum))
     else:
-        y, s, _ = ops.residual_norm_forward(x2, r2, gate, (kind_in, params[0], params[1], eps_in) if kind_in else None,
-                                            (kind_out, params[2], params[3], eps_out) if kind_out else None, float(alpha), p, state, call, bool(return_sum), want_stats=False)
+        y, s, _ = ops.residual_norm_forward(x2, r2, gate, (kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None,
+                                            alpha, p, state, call, return_sum, want_stats=False)
         res = (y, s) if kind_out and return_sum else (y if kind_out else s)
     return tuple(_shaped(t, shape) for t in res) if isinstance(res, tuple) else _shaped(res, shape)
 

@@ -6,9 +6,10 @@
 // An index outside [0, rows) names no row: it adds nothing and takes no gradient.  Sums in f32, rounded to the table's type once.
 //
 // The gradient: the entries that name a row are sorted by it (stable), cut into tiles of `tile` entries, and a group of lanes walks each tile, adding up
-// dout rows as long as the table row stays the same.  A row whose entries lie within one tile is written at once; one that crosses tiles leaves a
-// partial sum per tile, which k_emb_join adds in order.  So the work per group is the same whether every token is another one or all are the same, and
-// the order of the additions is fixed: no atomics on sums, the same bits every time.  Rows without entries: the table's gradient is cleared first.
+// dout rows as long as the table row stays the same.  The group in whose tile a row begins finishes it, into the next tile if need be; only a row that
+// covers a whole tile leaves a partial sum per tile, which k_emb_join adds in order.  So a group walks at most two tiles whether every token is another
+// one or all are the same, and the order of the additions is fixed: no atomics on sums, the same bits every time.  Rows without entries: the table's
+// gradient is cleared first.
 // Bound by memory: dout rows in, the whole gradient table out; the sort moves 8 bytes an entry and pass.
 #include "blocks_common.h"
 
@@ -16,8 +17,9 @@ __device__ __forceinline__ long long emb_index(const void *__restrict__ idx, int
   return is64 ? ((const long long *)idx)[e] : (long long)((const int32_t *)idx)[e];
 }
 
-// one chunk of 8 columns of one output row per thread and trip; four indices, then four table rows in flight.  I: 32 bits where the chunk count allows
-template <typename T, typename I>
+// One chunk of 8 columns of one output row per thread; I: 32 bits where the chunk count allows.  A lookup is a chain of two round trips (index, table row), so
+// several are kept in flight: U entries of a row that sums k > 1 of them, U rows of one entry each (grid-stride apart) for k = 1.
+template <typename T, typename I, int U>
 __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total, int k,
                                                  const float *__restrict__ weight, float scale, T *__restrict__ out) {
   const uint32_t groups = (uint32_t)(c + 7) / 8;
@@ -27,23 +29,24 @@ __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, si
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-    for (int q0 = 0; q0 < k; q0 += 4) {
-      long long v[4];
-      float w[4];
-      ls3d_raw8<T> r[4];
+    for (int q0 = 0; q0 < k; q0 += U) {
+      long long v[U];
+      float w[U];
+      ls3d_raw8<T> r[U];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < U; ++q) {
         const size_t e = (size_t)i * k + (q0 + q < k ? q0 + q : k - 1);
-        v[q] = q0 + q < k ? emb_index(idx, is64, e) : -1;
+        v[q] = emb_index(idx, is64, e);
         w[q] = weight ? weight[e] : 1.0f;
+        if (q0 + q >= k) v[q] = -1;
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < U; ++q) {
         r[q] = ls3d_raw8<T>{};
         if (v[q] >= 0 && v[q] < rows) r[q] = ls3d_load8<T>(table + (size_t)v[q] * table_ld, col, c);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < U; ++q) {
         if (v[q] < 0 || v[q] >= rows) continue;
         float x[8];
         ls3d_unpack8<T>(r[q], m, x);
@@ -57,11 +60,49 @@ __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, si
   }
 }
 
+template <typename T, typename I, int U>
+__global__ __launch_bounds__(256) void k_emb_fwd_one(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total,
+                                                     const float *__restrict__ weight, float scale, T *__restrict__ out) {
+  const uint32_t groups = (uint32_t)(c + 7) / 8;
+  const I step = (I)gridDim.x * 256;
+  for (I t0 = (I)blockIdx.x * 256 + threadIdx.x; t0 < total; t0 += step * U) {
+    uint32_t i[U], g[U];
+    long long v[U];
+    float w[U];
+    ls3d_raw8<T> r[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const I t = t0 + step * q < total ? t0 + step * q : t0;
+      i[q] = (uint32_t)(t / groups);
+      g[q] = (uint32_t)(t - (I)i[q] * groups);
+      v[q] = emb_index(idx, is64, i[q]);
+      w[q] = (weight ? weight[i[q]] : 1.0f) * scale;
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      r[q] = ls3d_raw8<T>{};
+      if (v[q] >= 0 && v[q] < rows) r[q] = ls3d_load8<T>(table + (size_t)v[q] * table_ld, (long long)g[q] * 8, c);
+    }
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      if (q > 0 && t0 + step * q >= total) break;
+      const int col = (int)g[q] * 8, m = c - col;
+      float x[8];
+      ls3d_unpack8<T>(r[q], m, x);
+      const bool hit = v[q] >= 0 && v[q] < rows;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = hit ? x[j] * w[q] : 0.0f;  // (a weight of NaN beside an index that names no row is not seen)
+      ls3d_store8<T>(out + (size_t)i[q] * c + col, x, m);
+    }
+  }
+}
+
 // ---- the entries sorted by table row: pairs (row, entry), stable, the entries without a row left out; *n_valid = how many there are.
 //      LSD radix passes of up to 11 bits (a table of up to 4 M rows: two), the first one straight from the indices.
-constexpr int ES_ITEMS = 16;              // entries a thread
-constexpr int ES_TILE = 256 * ES_ITEMS;   // entries a workgroup
 constexpr int ES_MAX_DIGITS = 2048;
+// entries per thread of a 256-thread workgroup: 16, or 4 where that leaves CUs without one
+static inline int es_items(long long entries) { return entries > 262144 ? 16 : 4; }
+static inline int es_tiles(long long entries) { return (int)((entries + 256 * es_items(entries) - 1) / (256 * es_items(entries))); }
 
 struct emb_keys { const void *idx; int is64; long long rows, padding; };  // where an entry's row comes from in the first pass
 __device__ __forceinline__ uint32_t emb_key(const emb_keys &K, size_t e) {  // 0xFFFFFFFF: no row
@@ -77,17 +118,17 @@ __device__ __forceinline__ void emb_clear(T *__restrict__ dtable, size_t elems, 
 }
 
 // per-workgroup digit counts -> hist[workgroup][digit]; FIRST: from the indices, and the gradient table is cleared by the same launch
-template <typename T, bool FIRST>
+template <typename T, bool FIRST, int ITEMS>
 __global__ __launch_bounds__(256) void k_es_hist(emb_keys K, const uint2 *__restrict__ pairs, int entries, const int32_t *__restrict__ n_valid, int shift, int digits, int ntiles,
                                                  int32_t *__restrict__ hist, T *__restrict__ dtable, size_t elems) {
   __shared__ int s_h[ES_MAX_DIGITS];
   if ((int)blockIdx.x < ntiles) {
     const int N = FIRST ? entries : *n_valid;
-    const long long lo = (long long)blockIdx.x * ES_TILE;
+    const long long lo = (long long)blockIdx.x * (256 * ITEMS);
     for (int d = threadIdx.x; d < digits; d += 256) s_h[d] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < ES_ITEMS; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       const long long e = lo + i * 256 + threadIdx.x;
       if (e < N) {
         const uint32_t key = FIRST ? emb_key(K, (size_t)e) : pairs[e].x;
@@ -166,23 +207,23 @@ __device__ __forceinline__ int emb_block_scan(int v, int *s_w, int *total) {
   return before + s - v;
 }
 
-// places a tile's items: a wave takes 64 * ES_ITEMS consecutive ones, 64 at a time; an item's rank among its wave's equal digits from ballots and a count per
+// places a tile's items: a wave takes 64 * ITEMS consecutive ones, 64 at a time; an item's rank among its wave's equal digits from ballots and a count per
 // wave and digit, the waves' and workgroups' shares on top.  Equal digits keep their order.
-template <bool FIRST>
+template <bool FIRST, int ITEMS>
 __global__ __launch_bounds__(256) void k_es_scatter(emb_keys K, const uint2 *__restrict__ pairs, int entries, int32_t *__restrict__ n_valid, int shift, int digits, int bits,
                                                     const int32_t *__restrict__ hist, const int32_t *__restrict__ totals, uint2 *__restrict__ out) {
   __shared__ int s_cnt[4][ES_MAX_DIGITS];
   __shared__ int s_w[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int N = FIRST ? entries : *n_valid;
-  const long long lo = (long long)blockIdx.x * ES_TILE;
+  const long long lo = (long long)blockIdx.x * (256 * ITEMS);
   if (lo >= N) return;  // (the first pass: every workgroup has items)
   for (int d = threadIdx.x; d < digits; d += 256) s_cnt[0][d] = s_cnt[1][d] = s_cnt[2][d] = s_cnt[3][d] = 0;
-  uint2 item[ES_ITEMS];
-  int rank[ES_ITEMS];
+  uint2 item[ITEMS];
+  int rank[ITEMS];
 #pragma unroll
-  for (int i = 0; i < ES_ITEMS; ++i) {
-    const long long e = lo + (wave * ES_ITEMS + i) * 64 + lane;
+  for (int i = 0; i < ITEMS; ++i) {
+    const long long e = lo + (wave * ITEMS + i) * 64 + lane;
     item[i].x = 0xFFFFFFFFu;
     item[i].y = (unsigned)e;
     if (e < N) {
@@ -192,7 +233,7 @@ __global__ __launch_bounds__(256) void k_es_scatter(emb_keys K, const uint2 *__r
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ES_ITEMS; ++i) {
+  for (int i = 0; i < ITEMS; ++i) {
     const bool live = item[i].x != 0xFFFFFFFFu;
     const uint32_t d = (item[i].x >> shift) & (uint32_t)(digits - 1);
     const unsigned long long peers = emb_peers(live, d, bits);
@@ -223,7 +264,7 @@ __global__ __launch_bounds__(256) void k_es_scatter(emb_keys K, const uint2 *__r
   if (FIRST && blockIdx.x == 0 && threadIdx.x == 0) *n_valid = total;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < ES_ITEMS; ++i)
+  for (int i = 0; i < ITEMS; ++i)
     if (item[i].x != 0xFFFFFFFFu) out[s_cnt[wave][(item[i].x >> shift) & (uint32_t)(digits - 1)] + rank[i]] = item[i];
 }
 
@@ -292,8 +333,10 @@ __global__ __launch_bounds__(1024) void k_es_small(emb_keys K, int entries, int 
   if (threadIdx.x == 0) *n_valid = total;
 }
 
-// grid (groups of tiles, column slabs): `lpr` lanes per tile, a chunk of 8 columns each; four entries' rows in flight
-template <typename T>
+// grid (groups of tiles, column slabs): `lpr` lanes per tile, a chunk of 8 columns each; U entries' rows in flight.
+// A row is LONG where it covers a whole tile; the sums of a long row's tiles go to partial[tile][0 | 1] (0: it began in an earlier tile).  A row that
+// begins in a tile and is not long is finished by that tile's group, and the next tile's group passes over its entries there.
+template <typename T, int U>
 __global__ __launch_bounds__(256) void k_emb_tiles(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int lpr, int c, int k,
                                                    const float *__restrict__ weight, float scale, const T *__restrict__ dout, size_t dout_ld,
                                                    T *__restrict__ dtable, float *__restrict__ partial) {
@@ -302,35 +345,48 @@ __global__ __launch_bounds__(256) void k_emb_tiles(const uint2 *__restrict__ pai
   const int col = ((int)blockIdx.y * lpr + lane) * 8, m = c - col;
   if (lo >= N || m <= 0) return;
   const int hi = lo + tile < N ? (int)(lo + tile) : N;
-  uint32_t cur = pairs[lo].x;
-  bool from_before = lo > 0 && pairs[lo - 1].x == cur;  // the open row began in an earlier tile
-  const bool goes_on = hi < N && pairs[hi < N ? hi : 0].x == pairs[hi - 1].x;
+  auto row_at = [&](long long e) { return e >= 0 && e < N ? pairs[e].x : 0xFFFFFFFFu; };  // (behind either end: no row has this number)
+  const uint32_t first = pairs[lo].x, last = pairs[hi - 1].x;
+  const uint32_t b1 = row_at(lo - 1), b2 = row_at(lo - tile - 1), n0 = row_at(hi), n1 = row_at((long long)hi + tile);
+  uint32_t cur = first;
+  bool from_before = b1 == first;                             // the open row began in an earlier tile,
+  bool skip = from_before && b2 != first && n0 != first;      // in the one before, whose group finishes it here (it covers neither that tile nor this one)
+  const bool spills = n0 == last && (hi - lo == tile);        // the last row goes on in the next tile,
+  const bool finish = spills && n1 != last && !(from_before && first == last);  // and ends there: this group goes after it
   float acc[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
-  for (int e0 = (int)lo; e0 < hi; e0 += 4) {
-    uint2 pr[4];
-    float w[4];
-    ls3d_raw8<T> r[4];
+  auto close = [&]() {  // the open row is complete
+    if (!skip) {
+      if (from_before) ls3d_store8<float>(partial + ((size_t)j * 2) * c + col, acc, m);
+      else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) pr[u] = pairs[e0 + u < hi ? e0 + u : hi - 1];
+        for (int q = 0; q < 8; ++q) acc[q] *= scale;
+        ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
+      }
+    }
+  };
+  const int end = finish ? (hi + tile < N ? hi + tile : N) : hi;
+  bool over = false;
+  for (int e0 = (int)lo; e0 < end && !over; e0 += U) {
+    uint2 pr[U];
+    float w[U];
+    ls3d_raw8<T> r[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) pr[u] = pairs[e0 + u < end ? e0 + u : end - 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       w[u] = weight ? weight[pr[u].y] : 1.0f;
       r[u] = ls3d_load8<T>(dout + (size_t)(k == 1 ? pr[u].y : pr[u].y / (unsigned)k) * dout_ld, col, c);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (e0 + u >= hi) continue;
+    for (int u = 0; u < U; ++u) {
+      if (e0 + u >= end || over) continue;
       if (pr[u].x != cur) {  // the same for every lane of the group
-        if (from_before) ls3d_store8<float>(partial + ((size_t)j * 2) * c + col, acc, m);
-        else {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] *= scale;
-          ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
-        }
+        if (e0 + u >= hi) { over = true; continue; }  // behind the tile: only the open row is followed
+        close();
         cur = pr[u].x;
-        from_before = false;
+        from_before = skip = false;
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
       }
@@ -340,61 +396,77 @@ __global__ __launch_bounds__(256) void k_emb_tiles(const uint2 *__restrict__ pai
       for (int q = 0; q < 8; ++q) acc[q] = fmaf(w[u], g[q], acc[q]);
     }
   }
-  if (from_before) ls3d_store8<float>(partial + ((size_t)j * 2) * c + col, acc, m);
-  else if (goes_on) ls3d_store8<float>(partial + ((size_t)j * 2 + 1) * c + col, acc, m);
-  else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] *= scale;
-    ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
-  }
+  if (spills && !finish && !from_before) ls3d_store8<float>(partial + ((size_t)j * 2 + 1) * c + col, acc, m);
+  else close();
 }
 
-// a workgroup for each tile in which a row begins that goes on in the next one: partial[j][1] + partial[j + 1][0] + ... while the tiles begin with that row.
-// `lpr` lanes per partial row, the 256 / lpr groups take the tiles in turn (one wave walking the 700 tiles of a row one after the other took 210 us), their
-// sums are added in order.
+// The long rows: partial[j][1] + partial[j + 1][0] + ... from the tile j in which the row begins, while the tiles begin with it.  A workgroup looks at EJ_TILES
+// tiles (few are such a j) and takes what it finds one after the other, all its threads together: `lpr` lanes per partial row, the 256 / lpr groups take the tiles in
+// turn (one wave walking the 700 tiles of a row one after the other took 210 us), their sums are added in order.
+constexpr int EJ_TILES = 16;
 template <typename T>
 __global__ __launch_bounds__(256) void k_emb_join(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int lpr, int c, float scale,
                                                   const float *__restrict__ partial, T *__restrict__ dtable) {
   __shared__ float s_sum[256][9];
-  const int j = (int)blockIdx.x, N = *n_valid;
-  const long long hi = (long long)(j + 1) * tile;
-  if (hi >= N) return;
-  const int ntiles = (int)(((long long)N + tile - 1) / tile);
-  const uint32_t cur = pairs[hi - 1].x;
-  if (pairs[hi].x != cur) return;  // nothing goes on (uniform over the workgroup, like the next line)
-  if (j > 0 && pairs[hi - tile].x == cur && pairs[hi - tile - 1].x == cur) return;  // it began in an earlier tile
-  int last = j + 1;  // the last tile that begins with this row: sorted, so those that do are the first of any run of tiles
-  for (;;) {
-    const long long t = (long long)last + 1 + threadIdx.x;
-    const int on = __syncthreads_count(t < ntiles && pairs[t < ntiles ? t * tile : 0].x == cur);
-    last += on;
-    if (on < 256) break;
+  __shared__ int s_begin[EJ_TILES], s_rest;
+  const int N = *n_valid;
+  const long long j0 = (long long)blockIdx.x * EJ_TILES, mine = (j0 + threadIdx.x + 1) * tile;  // `mine`: where this thread's tile ends
+  if (j0 * tile >= N) return;
+  bool begins = false;
+  if (threadIdx.x < EJ_TILES && mine + tile < N) {  // a long row that begins in the tile covers the next one and goes on (or ends) behind it
+    const uint32_t row = pairs[mine - 1].x;
+    begins = pairs[mine].x == row && pairs[mine + tile].x == row && !(mine > tile && pairs[mine - tile].x == row && pairs[mine - tile - 1].x == row);
   }
+  if (threadIdx.x < EJ_TILES) s_begin[threadIdx.x] = begins;
+  if (__syncthreads_count(begins) == 0) return;
   const int lane = (int)threadIdx.x % lpr, grp = (int)threadIdx.x / lpr, ngrp = 256 / lpr;
   const int col = ((int)blockIdx.y * lpr + lane) * 8, m = c - col;
-  float acc[8];
+  const int ntiles = (int)(((long long)N + tile - 1) / tile);
+  for (int q0 = 0; q0 < EJ_TILES; ++q0) {
+    if (!s_begin[q0]) continue;  // uniform
+    const int j = (int)j0 + q0;
+    const uint32_t cur = pairs[((long long)j + 1) * tile - 1].x;
+    int last = j + 1;  // the last tile that begins with this row: sorted, so those that do are the first of any run of tiles
+    for (;;) {  // 2048 tiles a step, a thread eight of them next to each other
+      int on = 0;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
-  if (m > 0) {
-#pragma unroll 4
-    for (int t = j + 1 + grp; t <= last; t += ngrp) {
-      float p[8];
-      ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)t * 2) * c, col, c), m, p);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] += p[q];
+      for (int u = 0; u < 8; ++u) {
+        const long long t = (long long)last + 1 + threadIdx.x * 8 + u;
+        on += t < ntiles && pairs[t < ntiles ? t * tile : 0].x == cur;
+      }
+      const int full = __syncthreads_count(on == 8), some = __syncthreads_count(on > 0);  // `some` threads, all but the last of them full
+      last += full * 8;
+      if (full == 256) continue;
+      if (some > full && (int)threadIdx.x == full) s_rest = on;
+      __syncthreads();
+      if (some > full) last += s_rest;
+      break;
     }
-  }
+    float acc[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) s_sum[threadIdx.x][q] = acc[q];
-  __syncthreads();
-  if (grp == 0 && m > 0) {
-    ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)j * 2 + 1) * c, col, c), m, acc);
-    for (int g = 0; g < ngrp; ++g)
+    for (int q = 0; q < 8; ++q) acc[q] = 0.0f;
+    if (m > 0) {
+#pragma unroll 8
+      for (int t = j + 1 + grp; t <= last; t += ngrp) {
+        float p[8];
+        ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)t * 2) * c, col, c), m, p);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] += s_sum[g * lpr + lane][q];
+        for (int q = 0; q < 8; ++q) acc[q] += p[q];
+      }
+    }
 #pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] *= scale;
-    ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
+    for (int q = 0; q < 8; ++q) s_sum[threadIdx.x][q] = acc[q];
+    __syncthreads();
+    if (grp == 0 && m > 0) {
+      ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)j * 2 + 1) * c, col, c), m, acc);
+      for (int g = 0; g < ngrp; ++g)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) acc[q] += s_sum[g * lpr + lane][q];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) acc[q] *= scale;
+      ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
+    }
+    __syncthreads();
   }
 }
 
@@ -447,27 +519,34 @@ extern "C" int ls3d_embedding_forward(const void *table, long long table_ld, lon
   if (!out || ((uintptr_t)out & (ls3d_dtype_size(dtype) - 1))) return LS3D_ERR_ARG;
   const long long total = (long long)n * ((c + 7) / 8);
   const int is64 = idx_dtype == LS3D_INDEX_I64;
-  const dim3 grid = ls3d_grid(total);
-  if (total < (1ll << 31))
-    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, uint32_t>), grid, dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (uint32_t)total, k, weight,
-                                        scale, (T *)out));
-  else
-    EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, unsigned long long>), grid, dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,
-                                        (unsigned long long)total, k, weight, scale, (T *)out));
+#define EMB_FWD(I_, U_)                                                                                                                                                   \
+  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, I_, U_>), ls3d_grid(total), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (I_)total, k, \
+                                      weight, scale, (T *)out))
+#define EMB_FWD_ONE(I_, U_)                                                                                                                                               \
+  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd_one<T, I_, U_>), ls3d_grid(total), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,         \
+                                      (I_)total, weight, scale, (T *)out))
+  if (total < (1ll << 30)) {  // (the strides on top stay below 2^32)
+    if (k == 1) EMB_FWD_ONE(uint32_t, 4);
+    else if (k <= 4) EMB_FWD(uint32_t, 4);
+    else EMB_FWD(uint32_t, 8);
+  } else if (k == 1) EMB_FWD_ONE(unsigned long long, 4);
+  else EMB_FWD(unsigned long long, 4);
+#undef EMB_FWD
+#undef EMB_FWD_ONE
   LS3D_RETURN_IF_LAUNCH_FAILED();
   return LS3D_OK;
 }
 
-// entries per tile: about 2^18 lanes at work on the tiles of a large call, but no fewer than 16 entries
+// entries per tile: the lanes of a large call fill the card four times over even if two thirds of its entries name no row; 8 to 64 entries
 static inline int emb_tile(long long entries, int c) {
   const long long want = entries * ((c + 7) / 8) / 262144;
-  int t = 16;
-  while (t < want && t < 4096) t *= 2;
+  int t = 8;
+  while (t < want && t < 64) t *= 2;
   return t;
 }
 
 // the sorting of a call: up to ES_SMALL entries in one workgroup, else radix passes of at most 11 bits, as even as they come
-constexpr int ES_SMALL = 16384;
+constexpr int ES_SMALL = 4096;
 static inline int emb_passes(int bits) { return (bits + 10) / 11; }
 
 struct emb_space { size_t pairs[2], partial, hist, totals, n_valid, bytes; };  // byte offsets in the workspace
@@ -480,7 +559,7 @@ static emb_space emb_layout(long long entries, int c) {
   s.totals = take(ES_MAX_DIGITS * 4);
   s.pairs[0] = take((size_t)entries * 8);
   s.pairs[1] = take(entries > ES_SMALL ? (size_t)entries * 8 : 0);
-  s.hist = take(entries > ES_SMALL ? (size_t)((entries + ES_TILE - 1) / ES_TILE) * ES_MAX_DIGITS * 4 : 0);
+  s.hist = take(entries > ES_SMALL ? (size_t)es_tiles(entries) * ES_MAX_DIGITS * 4 : 0);
   s.partial = take((size_t)((entries + tile - 1) / tile) * 2 * c * sizeof(float));
   s.bytes = at + 256;
   return s;
@@ -513,29 +592,28 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
   uint2 *buf[2] = {(uint2 *)(ws + S.pairs[0]), (uint2 *)(ws + S.pairs[1])};
   if (entries <= ES_SMALL) {
     const bool ok = entries <= 1024   ? emb_sort_small<T, 1>(K, entries, bits, n_valid, buf[0], dtable, elems, stream)
-                    : entries <= 4096 ? emb_sort_small<T, 4>(K, entries, bits, n_valid, buf[0], dtable, elems, stream)
-                                      : emb_sort_small<T, 16>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
+                                      : emb_sort_small<T, 4>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
     return ok ? buf[0] : nullptr;
   }
-  const int passes = emb_passes(bits), per = (bits + passes - 1) / passes, ntiles = (entries + ES_TILE - 1) / ES_TILE, digits = 1 << per;
+  const int passes = emb_passes(bits), per = (bits + passes - 1) / passes, ntiles = es_tiles(entries), digits = 1 << per, items = es_items(entries);
   const unsigned clear = ls3d_grid((long long)(elems / 8 + 1)).x;
+#define ES_PASS(FIRST_, ITEMS_, GRID_)                                                                                                                                  \
+  do {                                                                                                                                                                  \
+    hipLaunchKernelGGL((k_es_hist<T, FIRST_, ITEMS_>), dim3(GRID_), dim3(256), 0, stream, K, (const uint2 *)in, entries, (const int32_t *)n_valid, p * per, digits,      \
+                       ntiles, hist, dtable, elems);                                                                                                                    \
+    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 63) / 64)), dim3(1024), 0, stream, hist, ntiles, digits, totals);                                            \
+    hipLaunchKernelGGL((k_es_scatter<FIRST_, ITEMS_>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, n_valid, p * per, digits, per,       \
+                       (const int32_t *)hist, (const int32_t *)totals, out);                                                                                            \
+  } while (0)
   for (int p = 0; p < passes; ++p) {
     uint2 *out = buf[p & 1], *in = buf[1 - (p & 1)];
-    if (p == 0) {
-      hipLaunchKernelGGL((k_es_hist<T, true>), dim3((unsigned)ntiles > clear ? (unsigned)ntiles : clear), dim3(256), 0, stream, K, (const uint2 *)nullptr, entries,
-                         (const int32_t *)nullptr, 0, digits, ntiles, hist, dtable, elems);
-    } else {
-      hipLaunchKernelGGL((k_es_hist<T, false>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, (const int32_t *)n_valid, p * per, digits, ntiles,
-                         hist, dtable, elems);
-    }
-    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 63) / 64)), dim3(1024), 0, stream, hist, ntiles, digits, totals);
-    if (p == 0)
-      hipLaunchKernelGGL((k_es_scatter<true>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)nullptr, entries, n_valid, 0, digits, per, (const int32_t *)hist,
-                         (const int32_t *)totals, out);
-    else
-      hipLaunchKernelGGL((k_es_scatter<false>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, n_valid, p * per, digits, per, (const int32_t *)hist,
-                         (const int32_t *)totals, out);
+    const unsigned first = (unsigned)ntiles > clear ? (unsigned)ntiles : clear;
+    if (p == 0 && items == 4) ES_PASS(true, 4, first);
+    else if (p == 0) ES_PASS(true, 16, first);
+    else if (items == 4) ES_PASS(false, 4, (unsigned)ntiles);
+    else ES_PASS(false, 16, (unsigned)ntiles);
   }
+#undef ES_PASS
   return buf[(passes - 1) & 1];
 }
 
@@ -551,8 +629,9 @@ static int emb_table_gradient(const emb_keys &K, int entries, int c, int k, cons
   const dim3 grid((unsigned)((ntiles + 256 / lpr - 1) / (256 / lpr)), (unsigned)((groups + lpr - 1) / lpr));
   const int32_t *n_valid = (const int32_t *)(ws + S.n_valid);
   float *partial = (float *)(ws + S.partial);
-  hipLaunchKernelGGL((k_emb_tiles<T>), grid, dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, k, weight, scale, dout, dout_ld, dtable, partial);
-  if (ntiles > 1) hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)(ntiles - 1), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, scale, (const float *)partial, dtable);
+  hipLaunchKernelGGL((k_emb_tiles<T, 8>), grid, dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, k, weight, scale, dout, dout_ld, dtable, partial);
+  if (ntiles > 1)
+    hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)((ntiles + EJ_TILES - 1) / EJ_TILES), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, scale, (const float *)partial, dtable);
   return LS3D_OK;
 }
 

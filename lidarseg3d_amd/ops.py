@@ -1842,16 +1842,17 @@ def _row_view(t, name):
     """(pointer, row stride) of a 2-D tensor whose rows are contiguous; any row stride from the row's length on"""
     if t is None:
         return None, 0
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    (n, c), (ld, unit) = t.shape, t.stride()
+    if (c > 1 and unit != 1) or (n > 1 and ld < c):
         raise RuntimeError("%s: 2-D tensor with contiguous rows needed (shape %s, strides %s)" % (name, tuple(t.shape), t.stride()))
-    _device_ok(t)
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
-
-
-def _device_ok(t):
     if t.is_cuda == _SIM:
-        raise RuntimeError("hipsim test hook active: CPU tensors only" if _SIM else
-                           "lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % t.device)
+        _wrong_device(t)
+    return t.data_ptr(), ld if n > 1 else (c or 1)
+
+
+def _wrong_device(t):
+    raise RuntimeError("hipsim test hook active: CPU tensors only" if _SIM else
+                       "lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % t.device)
 
 
 def _addr(t):
@@ -1860,7 +1861,8 @@ def _addr(t):
         return None
     if not t.is_contiguous():
         raise RuntimeError("non-contiguous tensor passed to libls3d")
-    _device_ok(t)
+    if t.is_cuda == _SIM:
+        _wrong_device(t)
     return t.data_ptr()
 
 
@@ -1885,10 +1887,15 @@ def _call_on(t, fn, what, *args):
         check(rc, what)
 
 
+def _fresh(t):
+    """a new contiguous tensor of t's shape, type and device"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def dropout_forward(x, p, state, call, relu=False):
     """x [rows, c] (contiguous rows) -> y of its type: ls3d_dropout_forward; state: int64 [2] (seed, step) on the device"""
     _same_device(x, state)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _fresh(x)
     px, ld = _row_view(x, "x")
     _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ld, x.shape[0], x.shape[1],
              DTYPES[x.dtype], p, _addr(state), call, int(relu), _addr(y))
@@ -1897,8 +1904,7 @@ def dropout_forward(x, p, state, call, relu=False):
 
 def dropout_backward(dy, y, p, state, call, relu=False):
     """dx from dy [rows, c] and - relu - the forward's output y (ls3d_dropout_backward)"""
-    _same_device(dy, state, y)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dx = _fresh(dy)
     pd, ld = _row_view(dy, "dy")
     _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ld, _addr(y), dy.shape[0],
              dy.shape[1], DTYPES[dy.dtype], p, _addr(state), call, int(relu), _addr(dx))
@@ -1907,25 +1913,18 @@ def dropout_backward(dy, y, p, state, call, relu=False):
 
 def residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call):
     """ls3d_residual_norm_t; norm_in / norm_out: None or (kind 1 layer | 2 rms, weight, bias, eps); gate: None, [c] or [n, c]"""
-    d = _lib.ResidualNorm()
-    for dst, nm in ((d.in_, norm_in), (d.out, norm_out)):
-        if nm is not None:
-            dst.kind, dst.eps = nm[0], nm[3]
-            if nm[1] is not None:
-                dst.weight, dst.weight_dtype = _addr(nm[1]), DTYPES[nm[1].dtype]
-            if nm[2] is not None:
-                dst.bias, dst.bias_dtype = _addr(nm[2]), DTYPES[nm[2].dtype]
+    norms = [_lib.Norm() if nm is None else
+             _lib.Norm(_addr(nm[1]), _addr(nm[2]), nm[0], 0 if nm[1] is None else DTYPES[nm[1].dtype], 0 if nm[2] is None else DTYPES[nm[2].dtype], nm[3])
+             for nm in (norm_in, norm_out)]
+    kind, g, ld, gt = 0, None, 0, 0
     if gate is not None:
-        d.gate_dtype = DTYPES[gate.dtype]
+        gt = DTYPES[gate.dtype]
         if gate.dim() == 1:
-            d.gate_kind, d.gate, d.gate_ld = 1, _addr(gate), 0
+            kind, g = 1, _addr(gate)
         else:
-            d.gate_kind = 2
-            d.gate, d.gate_ld = _row_view(gate, "gate")
-    d.dtype, d.stream_dtype = DTYPES[x.dtype], DTYPES[(x if residual is None else residual).dtype]
-    d.alpha, d.p, d.call = alpha, p, call
-    d.state = _addr(state)
-    return d
+            kind, (g, ld) = 2, _row_view(gate, "gate")
+    dt = DTYPES[x.dtype]
+    return _lib.ResidualNorm(norms[0], norms[1], g, ld, _addr(state), dt, dt if residual is None else DTYPES[residual.dtype], kind, gt, alpha, p, call)
 
 
 def residual_norm_forward(x, residual=None, gate=None, norm_in=None, norm_out=None, alpha=1.0, p=0.0, state=None, call=0, want_sum=False, want_stats=True):
@@ -1933,8 +1932,8 @@ def residual_norm_forward(x, residual=None, gate=None, norm_in=None, norm_out=No
     n, c = x.shape
     _same_device(x, residual, gate, state, *[t for nm in (norm_in, norm_out) if nm is not None for t in nm[1:3]])
     d = residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call)
-    y = torch.empty((n, c), dtype=x.dtype, device=x.device) if norm_out is not None else None
-    s = torch.empty((n, c), dtype=(x if residual is None else residual).dtype, device=x.device) if want_sum or norm_out is None else None
+    y = _fresh(x) if norm_out is not None else None
+    s = _fresh(x if residual is None else residual) if want_sum or norm_out is None else None
     stats = torch.empty((n, 4), dtype=torch.float32, device=x.device) if want_stats else None
     px, x_ld = _row_view(x, "x")
     pr, r_ld = _row_view(residual, "residual")
@@ -1947,10 +1946,9 @@ def residual_norm_backward(x, residual, gate, norm_in, norm_out, alpha, p, state
     """gradients (x, residual, gate, in weight, in bias, out weight, out bias) - None where `want` (7 truth values) says so - of residual_norm_forward
     (ls3d_residual_norm_backward); dy / ds: the gradients of y and s, None where that output was not used"""
     n, c = x.shape
-    _same_device(x, residual, gate, state, stats, dy, ds)
     d = residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call)
     like = (x, residual, gate) + (norm_in[1:3] if norm_in is not None else (None, None)) + (norm_out[1:3] if norm_out is not None else (None, None))
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if w and t is not None else None for t, w in zip(like, want)]
+    grads = [_fresh(t) if w and t is not None else None for t, w in zip(like, want)]
     L = _L()
     ws = _ws(L.ls3d_residual_norm_workspace_bytes(n, c), x)
     (px, x_ld), (pr, r_ld), (py, y_ld), (ps, s_ld) = _row_view(x, "x"), _row_view(residual, "residual"), _row_view(dy, "dy"), _row_view(ds, "ds")
@@ -1972,9 +1970,8 @@ def embedding_forward(table, idx, weight=None, scale=1.0):
 
 def embedding_backward(table, idx, weight, scale, padding, dout, want_table=True, want_weight=False):
     """(gradient of the table, gradient of the weights) of embedding_forward, None where not wanted (ls3d_embedding_backward)"""
-    _same_device(table, idx, weight, dout)
     (n, k), (rows, c) = idx.shape, table.shape
-    dt = torch.empty((rows, c), dtype=table.dtype, device=table.device) if want_table else None
+    dt = _fresh(table) if want_table else None
     dw = torch.empty((n, k), dtype=torch.float32, device=table.device) if want_weight else None
     L = _L()
     ws = _ws(L.ls3d_embedding_workspace_bytes(n, k, c), table)

@@ -198,6 +198,8 @@ EMBEDDING = [
     (12, 1030, BF16, (70,), False, False, 32.0, "few"),
     (9, 64, F32, (1300,), False, False, 1.0, "one"),
     (2500, 3, F32, (5000,), False, False, 1.0, "uniform"),
+    (150, 5, F32, (4000,), False, False, 1.0, "runs"),
+    (64, 3, F32, (2000,), False, False, 1.0, "runs"),
     # more entries than one workgroup sorts: radix passes of one digit, of two, with entries that name no row
     (300, 2, F32, (16500,), False, False, 1.0, "uniform"),
     (9000, 3, F16, (17001,), False, False, 1.0, "uniform"),
@@ -212,6 +214,9 @@ def tensor(gen, *shape, dtype=F32, scale=1.0, shift=0.0, device="cpu"):
 def indices(gen, rows, shape, how, device, dtype=torch.int64):
     if how == "one":
         ix = torch.full(shape, rows - 1)
+    elif how == "runs":  # rows named 1, 2, ... 70 times: they begin, end and fill up at every place of a tile
+        ix = torch.repeat_interleave(torch.arange(rows), torch.arange(rows) % 70 + 1)[:shape[0]]
+        ix = torch.cat([ix, torch.randint(0, rows, (shape[0] - ix.numel(),), generator=gen)])[torch.randperm(shape[0], generator=gen)]
     elif how == "few":
         ix = torch.randint(0, min(rows, 3), shape, generator=gen)
     else:
