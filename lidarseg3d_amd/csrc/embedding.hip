@@ -100,8 +100,8 @@ __global__ __launch_bounds__(256) void k_emb_fwd_one(const T *__restrict__ table
 // ---- the entries sorted by table row: pairs (row, entry), stable, the entries without a row left out; *n_valid = how many there are.
 //      LSD radix passes of up to 11 bits (a table of up to 4 M rows: two), the first one straight from the indices.
 constexpr int ES_MAX_DIGITS = 2048;
-// entries per thread of a 256-thread workgroup: 16, or 4 where that leaves CUs without one
-static inline int es_items(long long entries) { return entries > 262144 ? 16 : 4; }
+// entries per thread of a 256-thread workgroup: 8, or 4 where that leaves CUs without one
+static inline int es_items(long long entries) { return entries > 1048576 ? 8 : 4; }
 static inline int es_tiles(long long entries) { return (int)((entries + 256 * es_items(entries) - 1) / (256 * es_items(entries))); }
 
 struct emb_keys { const void *idx; int is64; long long rows, padding; };  // where an entry's row comes from in the first pass
@@ -141,35 +141,35 @@ __global__ __launch_bounds__(256) void k_es_hist(emb_keys K, const uint2 *__rest
   if (FIRST) emb_clear<T>(dtable, elems, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
 
-// hist[workgroup][digit] -> the digit's count in the workgroups before, totals[digit]: 64 digits x 16 segments of workgroups per workgroup
+// hist[workgroup][digit] -> the digit's count in the workgroups before, totals[digit]: 32 digits x 32 segments of workgroups per workgroup
 __global__ __launch_bounds__(1024) void k_es_scan(int32_t *__restrict__ hist, int ntiles, int digits, int32_t *__restrict__ totals) {
-  __shared__ int s_seg[16][64];
-  const int d = blockIdx.x * 64 + (threadIdx.x & 63), seg = threadIdx.x >> 6, per = (ntiles + 15) / 16;
+  __shared__ int s_seg[32][33];
+  const int d = blockIdx.x * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5, per = (ntiles + 31) / 32;
   const int lo = seg * per, hi = lo + per < ntiles ? lo + per : ntiles;
   const bool on = d < digits;
   int s = 0;
-  for (int b = lo; b < hi; b += 8) {
-    int v[8];
+  for (int b = lo; b < hi; b += 16) {
+    int v[16];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
+    for (int q = 0; q < 16; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) s += v[q];
+    for (int q = 0; q < 16; ++q) s += v[q];
   }
-  s_seg[seg][threadIdx.x & 63] = s;
+  s_seg[seg][threadIdx.x & 31] = s;
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    const int x = s_seg[q][threadIdx.x & 63];
+  for (int q = 0; q < 32; ++q) {
+    const int x = s_seg[q][threadIdx.x & 31];
     before += q < seg ? x : 0;
     total += x;
   }
-  for (int b = lo; b < hi; b += 8) {
-    int v[8];
+  for (int b = lo; b < hi; b += 16) {
+    int v[16];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
+    for (int q = 0; q < 16; ++q) v[q] = on && b + q < hi ? hist[(size_t)(b + q) * digits + d] : 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
+    for (int q = 0; q < 16; ++q)
       if (on && b + q < hi) { hist[(size_t)(b + q) * digits + d] = before; before += v[q]; }
   }
   if (on && seg == 0) totals[d] = total;
@@ -601,7 +601,7 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
   do {                                                                                                                                                                  \
     hipLaunchKernelGGL((k_es_hist<T, FIRST_, ITEMS_>), dim3(GRID_), dim3(256), 0, stream, K, (const uint2 *)in, entries, (const int32_t *)n_valid, p * per, digits,      \
                        ntiles, hist, dtable, elems);                                                                                                                    \
-    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 63) / 64)), dim3(1024), 0, stream, hist, ntiles, digits, totals);                                            \
+    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 31) / 32)), dim3(1024), 0, stream, hist, ntiles, digits, totals);                                            \
     hipLaunchKernelGGL((k_es_scatter<FIRST_, ITEMS_>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, n_valid, p * per, digits, per,       \
                        (const int32_t *)hist, (const int32_t *)totals, out);                                                                                            \
   } while (0)
@@ -609,9 +609,9 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
     uint2 *out = buf[p & 1], *in = buf[1 - (p & 1)];
     const unsigned first = (unsigned)ntiles > clear ? (unsigned)ntiles : clear;
     if (p == 0 && items == 4) ES_PASS(true, 4, first);
-    else if (p == 0) ES_PASS(true, 16, first);
+    else if (p == 0) ES_PASS(true, 8, first);
     else if (items == 4) ES_PASS(false, 4, (unsigned)ntiles);
-    else ES_PASS(false, 16, (unsigned)ntiles);
+    else ES_PASS(false, 8, (unsigned)ntiles);
   }
 #undef ES_PASS
   return buf[(passes - 1) & 1];
