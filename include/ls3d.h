@@ -791,12 +791,13 @@ int ls3d_layer_norm_backward(const float *x, const float *dy, const float *gamma
 /* Dropout with a counter-based mask that is never stored.  Element (row, col) is dropped where its 16-bit draw is below t = round(65536 p), else scaled
  * by 65536 / (65536 - t) (p is thus resolved to 2^-16 and the expectation is x exactly; p = 1 drops all).  Draws: Philox4x32 with 10 rounds, key = seed,
  * counter = (col / 8, row, call, step), eight draws a counter, low half words first.  state = (seed, step), two int64 on the DEVICE (read when the kernel runs:
- * a captured graph draws anew when the step is advanced between replays); call: the call's number within a step.  relu: of relu(x).
- * A dropped element is 0 whatever x holds there.  backward: the same state, call and p; relu: y is the forward's output (else NULL). */
+ * a captured graph draws anew when the step is advanced between replays); call: the call's number within a step.  relu: of relu(x); bits
+ * [rows][(c + 7) / 8], a byte for 8 columns (may be NULL): which elements were kept and positive, for the backward pass (NULL there without relu).
+ * A dropped element is 0 whatever x holds there.  backward: the same state, call and p. */
 int ls3d_dropout_forward(const void *x, long long x_ld, long long rows, long long c, int dtype, float p, const int64_t *state, uint32_t call, int relu,
-                         void *y, ls3d_stream_t stream);
-int ls3d_dropout_backward(const void *dy, long long dy_ld, const void *y, long long rows, long long c, int dtype, float p, const int64_t *state, uint32_t call,
-                          int relu, void *dx, ls3d_stream_t stream);
+                         void *y, uint8_t *bits, ls3d_stream_t stream);
+int ls3d_dropout_backward(const void *dy, long long dy_ld, const uint8_t *bits, long long rows, long long c, int dtype, float p, const int64_t *state,
+                          uint32_t call, int relu, void *dx, ls3d_stream_t stream);
 
 /* The residual of a transformer block with the norms before and after it, in one pass:
  *   t = in(x);  s = alpha * residual + gate * dropout(t);  y = out(s)

@@ -118,7 +118,7 @@ def _configure(lib):
     # the training-block operators are called with plain integers (an argument object each would be a third of a small call's host time)
     P, ll, i, f, u, z = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_uint32, ctypes.c_size_t
     D = ctypes.POINTER(ResidualNorm)
-    for name, types in (("ls3d_dropout_forward", (P, ll, ll, ll, i, f, P, u, i, P, P)), ("ls3d_dropout_backward", (P, ll, P, ll, ll, i, f, P, u, i, P, P)),
+    for name, types in (("ls3d_dropout_forward", (P, ll, ll, ll, i, f, P, u, i, P, P, P)), ("ls3d_dropout_backward", (P, ll, P, ll, ll, i, f, P, u, i, P, P)),
                         ("ls3d_residual_norm_forward", (P, ll, P, ll, i, i, D, P, P, P, P)), ("ls3d_residual_norm_workspace_bytes", (i, i)),
                         ("ls3d_residual_norm_backward", (P, ll, P, ll, i, i, D, P, P, ll, P, ll, P, P, P, P, P, P, P, P, z, P)),
                         ("ls3d_embedding_forward", (P, ll, ll, i, i, P, i, i, i, P, f, P, P)), ("ls3d_embedding_workspace_bytes", (i, i, i)),

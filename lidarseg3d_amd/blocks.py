@@ -123,24 +123,22 @@ def _draw(p, state, call):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, state, call, relu):
-        y = _shaped(ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu), x.shape)
-        ctx.save_for_backward(state, y if relu else None)
+        y, bits = ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu, ctx.needs_input_grad[0])
+        ctx.save_for_backward(state, bits)
         ctx.args = (p, call, relu)
-        return y
+        return _shaped(y, x.shape)
 
     @staticmethod
     def backward(ctx, dy):
         _once("dropout")
-        state, y = ctx.saved_tensors
+        state, bits = ctx.saved_tensors
         p, call, relu = ctx.args
-        c = dy.shape[-1]
-        dx = ops.dropout_backward(_rows(dy, c), _rows(y, c) if relu else None, p, state, call, relu)
-        return _shaped(dx, dy.shape), None, None, None, None
+        return _shaped(ops.dropout_backward(_rows(dy, dy.shape[-1]), bits, p, state, call, relu), dy.shape), None, None, None, None
 
 
 def dropout(x, p, state, call=None, relu=False):
     """dropout(x) - relu: dropout(relu(x)) - over the last dimension's rows, the mask made from (seed, step, call, row, column) in the forward pass and
-    again in the backward pass: nothing is stored (relu: the output itself, which the next layer keeps anyway, says where the gradient goes).
+    again in the backward pass: it is never stored (relu: one bit per element says where x was positive and kept).
     p is resolved to 1 / 65536 and what is kept is scaled by the inverse of the resolved probability.  state: a DropoutState, or its tensor together with
     `call`; two dropouts of one step need different calls.  A dropped element is zero whatever stood there."""
     _on_device(x, "dropout")

@@ -1892,22 +1892,23 @@ def _fresh(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def dropout_forward(x, p, state, call, relu=False):
-    """x [rows, c] (contiguous rows) -> y of its type: ls3d_dropout_forward; state: int64 [2] (seed, step) on the device"""
+def dropout_forward(x, p, state, call, relu=False, want_bits=False):
+    """x [rows, c] (contiguous rows) -> (y of its type, bits): ls3d_dropout_forward; state: int64 [2] (seed, step) on the device.  bits (relu and
+    want_bits, else None): uint8 [rows, ceil(c / 8)], what dropout_backward needs to know of x"""
     _same_device(x, state)
     y = _fresh(x)
+    bits = torch.empty((x.shape[0], (x.shape[1] + 7) // 8), dtype=torch.uint8, device=x.device) if relu and want_bits else None
     px, ld = _row_view(x, "x")
-    _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ld, x.shape[0], x.shape[1],
-             DTYPES[x.dtype], p, _addr(state), call, int(relu), _addr(y))
-    return y
+    _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ld, x.shape[0], x.shape[1], DTYPES[x.dtype], p, _addr(state), call, int(relu), _addr(y), _addr(bits))
+    return y, bits
 
 
-def dropout_backward(dy, y, p, state, call, relu=False):
-    """dx from dy [rows, c] and - relu - the forward's output y (ls3d_dropout_backward)"""
+def dropout_backward(dy, bits, p, state, call, relu=False):
+    """dx from dy [rows, c] and - relu - the forward's bits (ls3d_dropout_backward)"""
     dx = _fresh(dy)
     pd, ld = _row_view(dy, "dy")
-    _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ld, _addr(y), dy.shape[0],
-             dy.shape[1], DTYPES[dy.dtype], p, _addr(state), call, int(relu), _addr(dx))
+    _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ld, _addr(bits), dy.shape[0], dy.shape[1], DTYPES[dy.dtype], p, _addr(state), call, int(relu),
+             _addr(dx))
     return dx
 
 

@@ -148,11 +148,11 @@ def test_argument_errors_of_the_c_entry_points():
     P = lambda t, off=0: ctypes.c_void_p(t.data_ptr() + off)
     u = ctypes.c_uint32(0)
     ok = lambda **k: L.ls3d_dropout_forward(k.get("x", P(x)), ll(k.get("ld", 8)), ll(k.get("rows", 8)), ll(8), k.get("dt", 0), f(k.get("p", 0.5)), k.get("st", P(st)), u,
-                                            0, k.get("y", P(y)), None)
+                                            0, k.get("y", P(y)), None, None)
     assert ok() == 0 and ok(rows=0, x=None, y=None, st=None) == 0
     for bad in (dict(ld=7), dict(rows=-1), dict(dt=3), dict(p=1.5), dict(p=float("nan")), dict(st=None), dict(st=P(st, 4)), dict(x=None), dict(y=None), dict(x=P(x, 2))):
         assert ok(**bad) == ARG, bad
-    assert L.ls3d_dropout_backward(P(x), ll(8), None, ll(8), ll(8), 0, f(0.5), P(st), u, 1, P(y), None) == ARG  # relu: the output is needed
+    assert L.ls3d_dropout_backward(P(x), ll(8), None, ll(8), ll(8), 0, f(0.5), P(st), u, 1, P(y), None) == ARG  # relu: the bits are needed
     d = _lib.ResidualNorm()
     d.out.kind, d.alpha = 1, 1.0
     stats, ws = torch.zeros(8, 4), torch.zeros(1 << 16, dtype=torch.uint8)
