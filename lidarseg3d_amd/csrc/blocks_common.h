@@ -34,13 +34,14 @@ template <typename T>
 struct ls3d_raw8 { ls3d_u32x4 q[sizeof(T) / 2]; };  // a chunk as it stands in memory
 
 // the chunk at column `col` of a row of c columns, whatever of it lies inside: where fewer than 8 columns are left the LAST 8 of the row are read instead
-// (one access at any width and no branch around it; ls3d_unpack8 moves them into place), and a chunk that lies behind the row reads them too.
-template <typename T>
+// (one access at any width and no branch around it; ls3d_unpack8 moves them into place), and a chunk that lies behind the row reads them too.  NT: a
+// non-temporal access of a 2-byte type.
+template <typename T, bool NT = false>
 __device__ __forceinline__ ls3d_raw8<T> ls3d_load8(const T *__restrict__ row, long long col, long long c) {
   ls3d_raw8<T> r;
   if (c >= 8) {
     const T *__restrict__ p = row + (col < c - 8 ? col : c - 8);
-    if (sizeof(T) == 2) r.q[0] = *(const ls3d_u32x4_a2 *)p;
+    if (sizeof(T) == 2) r.q[0] = NT ? __builtin_nontemporal_load((const ls3d_u32x4_a2 *)p) : *(const ls3d_u32x4_a2 *)p;
     else {
       r.q[0] = *(const ls3d_u32x4_a4 *)p;
       r.q[sizeof(T) / 2 - 1] = *(const ls3d_u32x4_a4 *)((const char *)p + 16);
@@ -73,7 +74,7 @@ __device__ __forceinline__ void ls3d_unpack8(const ls3d_raw8<T> &r, int m, float
 }
 
 // rounds to T once (to nearest, ties to even) and stores the live columns
-template <typename T>
+template <typename T, bool NT = false>
 __device__ __forceinline__ void ls3d_store8(T *__restrict__ p, const float (&v)[8], int m) {
   T t[8];
 #pragma unroll
@@ -81,8 +82,10 @@ __device__ __forceinline__ void ls3d_store8(T *__restrict__ p, const float (&v)[
   if (m >= 8) {
     ls3d_raw8<T> r;
     __builtin_memcpy(&r, t, sizeof(t));
-    if (sizeof(T) == 2) *(ls3d_u32x4_a2 *)p = r.q[0];
-    else {
+    if (sizeof(T) == 2) {
+      if (NT) __builtin_nontemporal_store(r.q[0], (ls3d_u32x4_a2 *)p);
+      else *(ls3d_u32x4_a2 *)p = r.q[0];
+    } else {
       *(ls3d_u32x4_a4 *)p = r.q[0];
       *(ls3d_u32x4_a4 *)((char *)p + 16) = r.q[sizeof(T) / 2 - 1];
     }
@@ -96,6 +99,49 @@ __device__ __forceinline__ void ls3d_store8(T *__restrict__ p, const float (&v)[
   }
 }
 
+// half a chunk, 4 columns of f32 in one 16-byte access; the same treatment of the row's end
+template <bool NT>
+__device__ __forceinline__ ls3d_u32x4 ls3d_load4(const float *__restrict__ row, int col, int c) {
+  if (c >= 4) {
+    const ls3d_u32x4_a4 *p = (const ls3d_u32x4_a4 *)(row + (col < c - 4 ? col : c - 4));
+    return NT ? __builtin_nontemporal_load(p) : *p;
+  }
+  float t[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = j >= 4 - c ? row[j - (4 - c)] : 0.0f;
+  ls3d_u32x4 r;
+  __builtin_memcpy(&r, t, sizeof(t));
+  return r;
+}
+__device__ __forceinline__ void ls3d_unpack4(const ls3d_u32x4 &r, int m, float *v) {
+  float t[4];
+  __builtin_memcpy(t, &r, sizeof(t));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = t[j];
+  if (m < 4) {
+    LS3D_OPAQUE(m);
+    const int s = m > 0 ? 4 - m : 4;
+#pragma unroll
+    for (int step = 4; step >= 1; step >>= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (s & step) ? (j + step < 4 ? v[j + step] : 0.0f) : v[j];
+  }
+}
+template <bool NT>
+__device__ __forceinline__ void ls3d_store4(float *__restrict__ p, const float *v, int m) {
+  if (m >= 4) {
+    ls3d_u32x4 r;
+    __builtin_memcpy(&r, v, 16);
+    if (NT) __builtin_nontemporal_store(r, (ls3d_u32x4_a4 *)p);
+    else *(ls3d_u32x4_a4 *)p = r;
+  } else if (m > 0) {
+    LS3D_OPAQUE(m);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < m) p[j] = v[j];
+  }
+}
+
 // a chunk of a parameter vector of any of the types; NULL reads as `otherwise`; zeros behind the end
 __device__ __forceinline__ void ls3d_param8(const void *__restrict__ p, int dtype, int col, int c, float otherwise, float (&v)[8]) {
   const int m = c - col;
@@ -105,6 +151,18 @@ __device__ __forceinline__ void ls3d_param8(const void *__restrict__ p, int dtyp
   } else if (dtype == LS3D_DTYPE_F32) ls3d_unpack8<float>(ls3d_load8<float>((const float *)p, col, c), m, v);
   else if (dtype == LS3D_DTYPE_BF16) ls3d_unpack8<ls3d_bf16>(ls3d_load8<ls3d_bf16>((const ls3d_bf16 *)p, col, c), m, v);
   else ls3d_unpack8<ls3d_f16>(ls3d_load8<ls3d_f16>((const ls3d_f16 *)p, col, c), m, v);
+}
+// half a chunk of one
+__device__ __forceinline__ void ls3d_param4(const void *__restrict__ p, int dtype, int col, int c, float otherwise, float *v) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = col + j < c ? otherwise : 0.0f;
+  } else if (dtype == LS3D_DTYPE_F32) ls3d_unpack4(ls3d_load4<false>((const float *)p, col, c), c - col, v);
+  else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = col + j >= c ? 0.0f : dtype == LS3D_DTYPE_BF16 ? (float)((const ls3d_bf16 *)p)[col + j] : (float)((const ls3d_f16 *)p)[col + j];
+  }
 }
 __device__ __forceinline__ void ls3d_param_store(void *__restrict__ p, int dtype, size_t i, float v) {
   if (dtype == LS3D_DTYPE_F32) ((float *)p)[i] = v;

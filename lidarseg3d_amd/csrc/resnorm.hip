@@ -2,6 +2,7 @@
 #include "resnorm.h"
 
 constexpr int RN_MAX_C = 8192;      // 512 lanes x 2 chunks of 8 columns, 1024 x 1
+constexpr long long RN_NT_BYTES = 256ll << 20;
 constexpr int RN_BWD_BLOCKS = 512;  // workgroups of a backward pass: two per CU; each writes one row of column sums
 
 // lanes and chunks per lane of a row: few lanes (few exchanges a sum, more rows a wave), two chunks each, three where that fills four lanes.  With a norm before or
@@ -79,11 +80,19 @@ static int rn_fill(const ls3d_residual_norm_t *d, const void *x, long long x_ld,
   return LS3D_OK;
 }
 
-static bool rn_launch(bool fwd, bool full, int dtype, int stream_dtype, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {
-  if (dtype == LS3D_DTYPE_F32) return ls3d_rn_launch_f32(fwd, full, a, lpr, vpt, blocks, stream);
+// Non-temporal accesses where a pass moves more than any cache keeps until the next one (256 MB) and every access of a wave covers whole lines of a row: 16 lanes or
+// more, and no f32 rows beside 2-byte ones.  Measured, without / with: 100000 x 256 f32 208 / 191 us forward and backward, 16384 x 4096 bf16 forward 110 / 103 (100
+// on up to 16384 workgroups instead of 2048); narrower rows, 360000 x 96: f32 226 / 233, bf16 125 / 136; under 256 MB, 16384 x 1024 bf16: 74 / 77.
+static inline bool rn_streams(const ls3d_residual_norm_t *d, int lpr, long long elems, int of_x, int of_stream) {
+  const long long bytes = elems * ((long long)ls3d_dtype_size(d->dtype) * of_x + (long long)ls3d_dtype_size(d->stream_dtype) * of_stream);
+  return d->dtype == d->stream_dtype && lpr >= 16 && bytes > RN_NT_BYTES;
+}
+
+static bool rn_launch(bool fwd, bool full, bool nt, int dtype, int stream_dtype, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {
+  if (dtype == LS3D_DTYPE_F32) return ls3d_rn_launch_f32(fwd, full, nt, a, lpr, vpt, blocks, stream);
   if (dtype == LS3D_DTYPE_BF16)
-    return stream_dtype == LS3D_DTYPE_F32 ? ls3d_rn_launch_bf16_f32(fwd, full, a, lpr, vpt, blocks, stream) : ls3d_rn_launch_bf16(fwd, full, a, lpr, vpt, blocks, stream);
-  return stream_dtype == LS3D_DTYPE_F32 ? ls3d_rn_launch_f16_f32(fwd, full, a, lpr, vpt, blocks, stream) : ls3d_rn_launch_f16(fwd, full, a, lpr, vpt, blocks, stream);
+    return stream_dtype == LS3D_DTYPE_F32 ? ls3d_rn_launch_bf16_f32(fwd, full, nt, a, lpr, vpt, blocks, stream) : ls3d_rn_launch_bf16(fwd, full, nt, a, lpr, vpt, blocks, stream);
+  return stream_dtype == LS3D_DTYPE_F32 ? ls3d_rn_launch_f16_f32(fwd, full, nt, a, lpr, vpt, blocks, stream) : ls3d_rn_launch_f16(fwd, full, nt, a, lpr, vpt, blocks, stream);
 }
 
 extern "C" int ls3d_residual_norm_forward(const void *x, long long x_ld, const void *residual, long long res_ld, int n, int c, const ls3d_residual_norm_t *d,
@@ -97,8 +106,9 @@ extern "C" int ls3d_residual_norm_forward(const void *x, long long x_ld, const v
   int lpr, vpt;
   const bool full = a.kind_in || a.gate_kind;
   rn_shape(c, full, &lpr, &vpt);
+  const bool nt = rn_streams(d, lpr, (long long)n * c, 1 + (a.y != nullptr) + (a.gate_kind == LS3D_GATE_FULL), (a.res != nullptr) + (a.s != nullptr));
   const int rows = rn_rows(lpr);
-  if (!rn_launch(true, full, d->dtype, d->stream_dtype, a, lpr, vpt, (int)ls3d_grid(((long long)n + rows - 1) / rows, 1).x, (hipStream_t)stream)) return LS3D_ERR_UNSUPPORTED;
+  if (!rn_launch(true, full, nt, d->dtype, d->stream_dtype, a, lpr, vpt, (int)ls3d_grid(((long long)n + rows - 1) / rows, 1, nt ? 16384 : 2048).x, (hipStream_t)stream)) return LS3D_ERR_UNSUPPORTED;
   LS3D_RETURN_IF_LAUNCH_FAILED();
   return LS3D_OK;
 }
@@ -106,11 +116,13 @@ extern "C" int ls3d_residual_norm_forward(const void *x, long long x_ld, const v
 extern "C" size_t ls3d_residual_norm_workspace_bytes(int n, int c) {
   if (n < 0 || c < 0 || c > RN_MAX_C) return 0;
   int lpr, vpt;
-  rn_shape(c, true, &lpr, &vpt);
-  const int full = rn_bwd_blocks(n, lpr);
-  rn_shape(c, false, &lpr, &vpt);
-  const int simple = rn_bwd_blocks(n, lpr);
-  return (size_t)(full > simple ? full : simple) * 5 * c * sizeof(float) + 256;
+  int blocks = 0;  // of the shape with the fewest rows a workgroup
+  for (int full = 0; full < 2; ++full) {
+    rn_shape(c, full != 0, &lpr, &vpt);
+    const int b = rn_bwd_blocks(n, lpr);
+    blocks = b > blocks ? b : blocks;
+  }
+  return (size_t)blocks * 5 * c * sizeof(float) + 256;
 }
 
 extern "C" int ls3d_residual_norm_backward(const void *x, long long x_ld, const void *residual, long long res_ld, int n, int c, const ls3d_residual_norm_t *d,
@@ -149,8 +161,10 @@ extern "C" int ls3d_residual_norm_backward(const void *x, long long x_ld, const 
     int lpr, vpt;
     const bool full = a.kind_in || a.gate_kind;
     rn_shape(c, full, &lpr, &vpt);
+    const bool nt = rn_streams(d, lpr, (long long)n * c, 1 + (dy != nullptr) + (dx != nullptr) + (a.gate_kind == LS3D_GATE_FULL) + (a.dgate != nullptr),
+                      (a.res != nullptr) + (ds != nullptr) + (dresidual != nullptr));
     blocks = rn_bwd_blocks(n, lpr);
-    if (!rn_launch(false, full, d->dtype, d->stream_dtype, a, lpr, vpt, blocks, stream)) return LS3D_ERR_UNSUPPORTED;
+    if (!rn_launch(false, full, nt, d->dtype, d->stream_dtype, a, lpr, vpt, blocks, stream)) return LS3D_ERR_UNSUPPORTED;
   }
   if (nsum) hipLaunchKernelGGL(k_resnorm_columns, dim3((unsigned)((c + 31) / 32), (unsigned)nsum), dim3(1024), 0, stream, (const float *)workspace, blocks, nsum, c, o);
   LS3D_RETURN_IF_LAUNCH_FAILED();

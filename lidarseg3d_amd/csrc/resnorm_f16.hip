@@ -1,6 +1,6 @@
 // resnorm_f16.hip — the residual-norm kernels (resnorm.h) of one pair of element types: x, y as ls3d_f16, residual and sum as ls3d_f16.
 #include "resnorm.h"
 
-bool ls3d_rn_launch_f16(bool fwd, bool full, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {
-  return ls3d_rn_launch_types<ls3d_f16, ls3d_f16>(fwd, full, a, lpr, vpt, blocks, stream);
+bool ls3d_rn_launch_f16(bool fwd, bool full, bool nt, const ls3d_rn_args &a, int lpr, int vpt, int blocks, hipStream_t stream) {
+  return ls3d_rn_launch_types<ls3d_f16, ls3d_f16>(fwd, full, nt, a, lpr, vpt, blocks, stream);
 }

@@ -164,3 +164,38 @@ def test_large_table_and_offsets_beyond_32_bits():
     del z
     s, t = blocks.residual_norm(table.detach(), norm=blocks.Norm("rms"), p=0.5, state=st.tensor, call=0, return_sum=True)[::-1]
     assert torch.equal(s[rows - 64:], big)
+
+
+def test_large_passes_equal_their_parts():
+    """passes of more than 256 MB take other accesses (non-temporal, more workgroups): bit for bit what their parts give, row by row"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for n, c, T, kind in ((120001, 256, torch.float32, "layer"), (30001, 2050, torch.bfloat16, "rms"), (8193, 8191, torch.float16, "layer")):
+        x, r, dy = (torch.randn(n, c, generator=gen, device=DEV).to(T) for _ in range(3))
+        w = torch.randn(c, generator=gen, device=DEV, requires_grad=True)
+        parts = [slice(a, min(a + n // 5, n)) for a in range(0, n, n // 5)]
+
+        def run(sl, gate):
+            xs, rs = x[sl].detach().requires_grad_(), r[sl].detach().requires_grad_()
+            out = blocks.residual_norm(xs, rs, norm=blocks.Norm(kind, w), norm_in=blocks.Norm("rms", w) if gate else None, gate=w if gate else None, alpha=0.5, return_sum=True)
+            return [t.detach() for t in out] + list(torch.autograd.grad(out, [xs, rs, w], [dy[sl], dy[sl]]))
+        for gate in (False, True):
+            whole, pieces = run(slice(0, n), gate), [run(sl, gate) for sl in parts]
+            for i in range(4):
+                assert torch.equal(whole[i], torch.cat([p[i] for p in pieces])), (n, c, T, gate, i)
+            if not gate:  # dw = sum dy shat, here in float64 from the sum's values; terms added in f32, a thread's share of at most ceil(n / 512) + 64 in sequence
+                s = whole[1].double()
+                d = s - (s.mean(1, keepdim=True) if kind == "layer" else 0.0)
+                terms = dy.double() * d / (d.square().mean(1, keepdim=True) + 1e-5).sqrt()
+                # shat itself: K32 of the largest (|alpha r| + |x|) / std of a row, and the sum's rounding to its type
+                off = (dy.double().abs() * (bc.K32 * 8 + bc.unit(T) * s.abs().amax(1, keepdim=True))).sum(0)
+                assert bool(((whole[4].double() - terms.sum(0)).abs() <= (n / 512 + 64) * 2.0 ** -24 * terms.abs().sum(0) + off).all())
+            del whole, pieces
+        st = blocks.DropoutState(3, device=DEV)
+        big = torch.cat([x, r, dy]) if T != torch.float32 else torch.cat([x, r])
+        z = blocks.dropout(big, 0.3, st.tensor, call=5, relu=True)
+        keep, inv = bc.keep_mask(64, c, 0.3, 3, 0, 5)
+        want = torch.where(keep.to(DEV), torch.relu(big[:64].float()) * float(torch.tensor(inv, dtype=torch.float32)), torch.zeros((), device=DEV)).to(T)
+        assert torch.equal(z[:64], want)
+        assert torch.equal(z[:9000], blocks.dropout(big[:9000], 0.3, st.tensor, call=5, relu=True))
+        del big, z
