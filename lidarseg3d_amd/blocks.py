@@ -154,14 +154,16 @@ def dropout(x, p, state, call=None, relu=False):
 
 
 class Dropout(nn.Dropout):
-    """nn.Dropout on `dropout` with a DropoutState; evaluation passes its input through"""
+    """nn.Dropout on `dropout` with a DropoutState (None: torch's generator, as nn.Dropout); evaluation passes its input through"""
 
-    def __init__(self, p, state):
+    def __init__(self, p, state=None):
         super().__init__(p)
         self.state = state
 
     def forward(self, input):
-        return dropout(input, self.p, self.state) if self.training and self.p > 0 else input
+        if self.state is None:
+            return super().forward(input)
+        return dropout(input, self.p, self.state) if self.training else input
 
 
 # ---------------------------------------------------------------------------------------------- residual, dropout, gate and norms
@@ -185,8 +187,15 @@ class _ResidualNorm(torch.autograd.Function):
         if dy is None and ds is None:
             return (None,) * 9
         c = x.shape[1]
+        want = list(ctx.needs_input_grad[:7])
+        # s = residual + x: one gradient for both, written once
+        same = want[0] and want[1] and residual is not None and gate is None and not kind_in and p == 0.0 and alpha == 1.0 and x.dtype == residual.dtype
+        if same:
+            want[0] = False
         out = ops.residual_norm_backward(x, residual, gate, (kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None,
-                                         alpha, p, state, call, stats, None if dy is None else _rows(dy, c), None if ds is None else _rows(ds, c), ctx.needs_input_grad[:7])
+                                         alpha, p, state, call, stats, None if dy is None else _rows(dy, c), None if ds is None else _rows(ds, c), want)
+        if same:
+            out[0] = out[1]
         return (*out, None, None)
 
 
@@ -300,3 +309,24 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
     else:
         out = ops.embedding_forward(tab, flat, wgt, float(scale))
     return out if len(lead) == 1 else out.reshape(*lead, table.shape[1])
+
+
+# ---------------------------------------------------------------------------------------------- the models' training forward
+def use_in_training(model, state):
+    """Puts the training forward of a model of this package on the operators above: the SF-Phase decoder's and the TransVFE layers' residuals, dropouts and
+    norms in one pass each, dropout (the decoder's and the heads' nn.Dropout) from `state`, a DropoutState, and the camera features' sampling on one
+    weighted lookup.  The masks differ from torch's generator's (which still draws the class tokens' attention dropout inside nn.MultiheadAttention), everything
+    else agrees to rounding; evaluation is not touched.  The training loop
+    calls state.advance() after each backward pass.  state None: back to the torch composition.  -> model"""
+    if state is not None and not isinstance(state, DropoutState):
+        raise TypeError("use_in_training: a DropoutState or None needed, got %s" % type(state).__name__)
+    for module in list(model.modules()):
+        if hasattr(type(module), "block_state"):
+            module.block_state = state
+        if isinstance(module, Dropout):
+            module.state = state
+        for name, child in list(module.named_children()):
+            if type(child) is nn.Dropout and state is not None:
+                child = Dropout(child.p, state).train(child.training)
+                setattr(module, name, child)
+    return model

@@ -13,7 +13,7 @@ from functools import partial
 import torch
 from torch import nn
 
-from . import ops
+from . import blocks, ops
 from .packing import PackedModule, pack_linear
 from .registry import POINT_HEADS
 
@@ -343,6 +343,7 @@ def set_fused_sffm_memory(on):
 class SemanticFeatureFusionModule(PackedModule):
     """SFFM (context_module.py:56-117): points attend to the 2*num_cls class embeddings (camera + LiDAR) of their
     frame through num_decoder_layers post-norm decoder layers; the embeddings self-attend between layers."""
+    block_state = None  # blocks.use_in_training
 
     def __init__(self, d_input_point, d_input_embeddings1, d_input_embeddings2, embeddings_proj_kernel_size=1,
                  d_model=512, nhead=8, num_decoder_layers=6, dim_feedforward=2048, dropout=0.0, activation="relu",
@@ -541,8 +542,15 @@ def _sffm_forward_train(self, x, emb1, emb2, batch_idx, batch_size, return_conte
     mem = mem.permute(2, 0, 1).contiguous()  # [L, B, E]
     L = mem.shape[0]
     for l in self.decoder.layers:
-        drop = lambda t: F.dropout(t, l.dropout_p, self.training)
-        mem = l.norm1(mem + drop(l.self_attn(mem, mem, value=mem)[0]))
+        p = l.dropout_p if self.training else 0.0
+        if self.block_state is None:
+            drop = lambda t: F.dropout(t, p, self.training)
+            join = lambda t, x, norm: norm(t + drop(x))
+            act = lambda t: drop(F.relu(t))
+        else:  # dropout, residual and norm in one pass each (blocks.use_in_training)
+            join = lambda t, x, norm: blocks.residual_norm(x, t, norm=blocks.Norm.of(norm), p=p, state=self.block_state)
+            act = lambda t: blocks.dropout(t, p, self.block_state, relu=True)
+        mem = join(mem, l.self_attn(mem, mem, value=mem)[0], l.norm1)
         ca = l.crossocr_attn
         q = ca.q_proj(tgt).view(-1, H, hd)
         kv_in = mem.permute(1, 2, 0)  # [B, E, L]; the [B,E,L] result is then VIEWED as [B,H,hd,L] like the reference
@@ -555,8 +563,8 @@ def _sffm_forward_train(self, x, emb1, emb2, batch_idx, batch_size, return_conte
                 att = torch.softmax(torch.einsum("nhd,hdl->nhl", q[off[b]:off[b + 1]], k[b]) * hd ** -0.5, dim=-1)
                 rows.append(torch.einsum("nhl,hdl->nhd", att, v[b]))
             att_out = torch.cat(rows, 0)
-        tgt = l.norm2(tgt + drop(ca.out_proj(att_out.reshape(-1, H * hd))))
-        tgt = l.norm3(tgt + drop(l.linear2(drop(F.relu(l.linear1(tgt))))))
+        tgt = join(tgt, ca.out_proj(att_out.reshape(-1, H * hd)), l.norm2)
+        tgt = join(tgt, l.linear2(act(l.linear1(tgt))), l.norm3)
     tgt = self.decoder.norm_tgt(tgt)
     return (tgt, mem) if return_context else tgt
 
@@ -564,15 +572,16 @@ def _sffm_forward_train(self, x, emb1, emb2, batch_idx, batch_size, return_conte
 SemanticFeatureFusionModule._forward_train = _sffm_forward_train
 
 
-def _sample_image_rows(image_features, cuv, batch_idx):
+def _sample_image_rows(image_features, cuv, batch_idx, lookup=False):
     """get_points_image_feature (point_seg_mseg3d_head.py:200-236) under autograd: the 5-D bilinear grid_sample
-    (align_corners=True, zeros padding) written as 8 weighted row gathers from the channels-last maps, all frames at once"""
+    (align_corners=True, zeros padding) written as 8 weighted row gathers from the channels-last maps, all frames at once;
+    lookup: as one weighted row lookup (blocks.embedding), the maps' gradient sorted and added in a fixed order instead of eight scatters"""
     B, ncam, C, h, w = image_features.shape
     rows = image_features.permute(0, 1, 3, 4, 2).reshape(-1, C)
     pos = [(cuv[:, 1] + 1) * 0.5 * (ncam - 1), (cuv[:, 2] + 1) * 0.5 * (h - 1), (cuv[:, 3] + 1) * 0.5 * (w - 1)]
     lim = [ncam, h, w]
     lo = [p.floor() for p in pos]
-    out = image_features.new_zeros((cuv.shape[0], C))
+    out, entries, weights = None if lookup else image_features.new_zeros((cuv.shape[0], C)), [], []
     for corner in range(8):
         wgt, inside, cell = 1.0, True, []
         for a in range(3):
@@ -582,12 +591,18 @@ def _sample_image_rows(image_features, cuv, batch_idx):
             inside = (c >= 0) & (c <= lim[a] - 1) & inside
             cell.append(c.clamp(0, lim[a] - 1).long())
         flat = ((batch_idx.long() * ncam + cell[0]) * h + cell[1]) * w + cell[2]
-        out = out + rows[flat] * (wgt * inside).unsqueeze(1)
-    return out
+        if lookup:
+            entries.append(torch.where(inside & (wgt != 0), flat, torch.full_like(flat, -1)))
+            weights.append(wgt)
+        else:
+            out = out + rows[flat] * (wgt * inside).unsqueeze(1)
+    return blocks.embedding(rows, torch.stack(entries, 1), weight=torch.stack(weights, 1)) if lookup else out
 
 
 @POINT_HEADS.register_module
 class PointSegMSeg3DHead(PackedModule):
+    block_state = None  # blocks.use_in_training
+
     def __init__(self, class_agnostic, num_class, model_cfg, **kwargs):
         super().__init__()
         self.num_class = 1 if class_agnostic else num_class
@@ -672,7 +687,7 @@ class PointSegMSeg3DHead(PackedModule):
         pl = self.gffm_lidar(_interpolate_train(vf, idx, w, points, vx_off))
         cuv = batch_dict["points_cuv"]
         valid = cuv[:, 0] == 1
-        pc = self.gffm_camera(_sample_image_rows(batch_dict["image_features"], cuv[valid], points[:, 0][valid]))
+        pc = self.gffm_camera(_sample_image_rows(batch_dict["image_features"], cuv[valid], points[:, 0][valid], self.block_state is not None))
         ppc = self.lidar_camera_mimic_layer(pl[valid])
         # completed camera features (:320-334): rows without a camera hit stay zero, the pseudo-camera branch only
         # exists on the rows WITH a hit and feeds nothing but the mimic loss

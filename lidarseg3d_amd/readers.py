@@ -6,7 +6,7 @@ the MFMA gather-GEMM (csrc/spconv.hip) for every projection."""
 import torch
 from torch import nn
 
-from . import ops
+from . import blocks, ops
 from .packing import PackedModule, pack_linear
 from .registry import READERS
 
@@ -69,6 +69,7 @@ class TransformerVoxelFeatureExtractor(PackedModule):
     """TransVFE (voxel_encoder.py:166-270): per voxel, its <=5 points are tokens [point feats | descriptor];
     Conv1d(k=1) embed -> num_layers x pre-norm transformer layers (residual taken from the NORMED tensor,
     :154-161, no padding mask) -> max over the tokens -> Linear+ReLU compression."""
+    block_state = None  # blocks.use_in_training
 
     def __init__(self, num_input_features=4, num_compressed_features=16, num_embed=64, num_head=4, num_layers=2,
                  norm_cfg=None, name="TransformerVoxelFeatureExtractor"):
@@ -136,11 +137,19 @@ class TransformerVoxelFeatureExtractor(PackedModule):
         tok = ops.vfe_tokens(features.contiguous(), num_voxels.to(torch.int32).contiguous(), (kt + 15) // 16 * 16)[:, :kt]
         conv = self.feature_conv[0]
         x = torch.nn.functional.linear(tok, conv.weight.squeeze(-1), conv.bias).view(V, P, self.num_embed).permute(1, 0, 2)
-        for l in self.chunck.layers:  # voxel_encoder.py:149-163: the residuals start from the NORMED tensor
-            x = l.norm1(x)
-            x = x + l.self_attn(x, x, x, need_weights=False)[0]
-            x = l.norm2(x)
-            x = x + l.linear2(torch.relu(l.linear1(x)))
+        if self.block_state is None or not len(self.chunck.layers):
+            for l in self.chunck.layers:  # voxel_encoder.py:149-163: the residuals start from the NORMED tensor
+                x = l.norm1(x)
+                x = x + l.self_attn(x, x, x, need_weights=False)[0]
+                x = l.norm2(x)
+                x = x + l.linear2(torch.relu(l.linear1(x)))
+        else:  # a sub-layer's output, the residual and the next norm in one pass (blocks.use_in_training; the layers have no dropout)
+            layers = self.chunck.layers
+            x = layers[0].norm1(x)
+            for i, l in enumerate(layers):
+                x = blocks.residual_norm(l.self_attn(x, x, x, need_weights=False)[0], x, norm=blocks.Norm.of(l.norm2))
+                after = blocks.Norm.of(layers[i + 1].norm1) if i + 1 < len(layers) else None
+                x = blocks.residual_norm(l.linear2(torch.relu(l.linear1(x))), x, norm=after)
         x = x.max(dim=0)[0]
         return self.compress_layer(x) if self.compress_layer is not None else x
 

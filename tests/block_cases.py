@@ -164,6 +164,8 @@ RESIDUAL_NORM = [
     (70, 8, BF16, BF16, "layer", None, "channel", 1.0, 0.5, True),
     (66, 33, F16, F16, "layer", "rms", None, 0.5, 0.1, False),
     (131, 96, F32, F32, "layer", None, None, 1.0, 0.1, False),
+    (13, 96, F32, F32, "layer", None, None, 1.0, 0.0, True),
+    (14, 200, BF16, BF16, "rms", None, None, 1.0, 0.0, False),
     (9, 96, BF16, F32, None, "layer", "channel", 1.0, 0.25, True),
     (17, 128, F16, F32, "rms", "rms", "full", 1.0, 0.0, True),
     (20, 129, F32, F32, "rms", None, "channel", -1.0, 0.2, True),
@@ -453,3 +455,99 @@ def run_block(device, rows, width, table):
     val = lambda e: sum(float((o * w.cpu().double()).sum()) for o, w in zip(plain({k: Q[k].detach() + e * dirs[k] for k in Q}), (dy, ds)))
     slope, along = (val(1e-6) - val(-1e-6)) / 2e-6, sum(float((g.cpu().double() * dirs[k]).sum()) for k, g in zip(Q, grads))
     assert abs(slope - along) <= 1e-4 * sum(float((g.cpu().double() * dirs[k]).abs().sum()) for k, g in zip(Q, grads))
+
+
+def run_decoder(device, points, p, monkeypatch, frames=2, classes=17):
+    """the SF-Phase decoder's training forward on the block operators against its torch composition with the same masks: F.dropout of the composition is
+    given the operators' draws (same step, same order of calls)"""
+    from lidarseg3d_amd import blocks, point_heads
+    torch.manual_seed(1)
+    m = point_heads.SemanticFeatureFusionModule(64, 48, 32, d_model=96, nhead=4, num_decoder_layers=2, dim_feedforward=192, dropout=p).to(device).train()
+    for l in m.decoder.layers:  # the dropout of the class tokens' attention weights stays torch's in both forms
+        l.self_attn.dropout = 0.0
+    gen = torch.Generator().manual_seed(2)
+    x = tensor(gen, points, 64, device=device).requires_grad_()
+    e1, e2 = tensor(gen, frames, 48, classes, 1, device=device).requires_grad_(), tensor(gen, frames, 32, classes, 1, device=device).requires_grad_()
+    batch = (torch.arange(points) * frames // points).float().to(device)
+    dy = tensor(gen, points, 96, device=device)
+    leaves = [x, e1, e2] + list(m.parameters())
+
+    def run(state):
+        blocks.use_in_training(m, state)
+        y = m(x, e1, e2, batch, frames)
+        return [y.detach()] + [g for g in torch.autograd.grad(y, leaves, [dy], allow_unused=True)]
+    got = run(blocks.DropoutState(5, device=device, step=3))
+    draws = blocks.DropoutState(5, device=device, step=3)
+    monkeypatch.setattr(torch.nn.functional, "dropout", lambda t, q=0.5, training=True, inplace=False: blocks.dropout(t, q, draws) if training and q > 0 else t)
+    want = run(None)
+    assert len(got) == len(want)
+    # The scale of a gradient is the largest gradient of any leaf, not its own: a key projection's bias moves all scores of a query alike, softmax does not see
+    # it, and its gradient is an exact zero in the formulas: what is computed is the rounding of a sum whose terms (the keys' gradients, which also make up the
+    # projection's weight gradient) are as large as the other leaves' and cancel.
+    top = max(float(w.abs().max()) for w in want[1:] if w is not None)
+    for i, (g, w) in enumerate(zip(got, want)):
+        assert (g is None) == (w is None)
+        if g is not None:
+            # two float32 evaluations of the same formulas: 2 layers of 4 products (at most 192 terms), 3 norms each; K32 per norm and product
+            rel = 2 * 2 * 7 * K32
+            if i == 0 or points <= 1000:
+                bound = rel * (float(w.abs().max()) if i == 0 else top)
+                assert float((g - w).abs().max()) <= bound, (i, float((g - w).abs().max()), bound)
+            elif w.dim() > 1:
+                # Many points: a ReLU whose input is within its error of zero may open in one evaluation and not in the other, and an element of a gradient then
+                # jumps.  The inputs a (LayerNorm rows times W1, entries +-1 / sqrt(96): deviation 0.58, density at most 0.4 / 0.58, |a| <= 3) are off by
+                # at most rel / 2 * 3, so a share f <= 2 (rel / 2 * 3) 0.7 of the gates may differ; the hidden gradient's norm moves by sqrt(f), twice
+                # for two layers.  (A wrong mask at p = 0.1 moves it by sqrt(0.18) = 0.42.)
+                f = 2 * (rel / 2 * 3) * 0.7
+                assert float((g - w).norm()) <= (rel + 2 * f ** 0.5) * float(w.norm()), (i, float((g - w).norm() / w.norm()))
+
+
+def run_reader(device, voxels):
+    """the TransVFE reader's training forward on the block operators against its torch composition (no dropout there)"""
+    from lidarseg3d_amd import blocks, readers
+    torch.manual_seed(3)
+    m = readers.TransformerVoxelFeatureExtractor(num_input_features=5, num_layers=2).to(device).train()
+    gen = torch.Generator().manual_seed(4)
+    v, n = tensor(gen, voxels, 5, 5, device=device), (torch.arange(voxels) % 5 + 1).to(torch.int32).to(device)
+    res = []
+    for state in (None, blocks.DropoutState(1, device=device)):
+        y = blocks.use_in_training(m, state)(v, n)
+        res.append([y.detach()] + list(torch.autograd.grad(y, list(m.parameters()), [torch.ones_like(y)])))
+    for w, g in zip(*res):
+        assert float((g - w).abs().max()) <= 2 * 2 * 6 * K32 * max(float(w.abs().max()), 1e-3), (float((g - w).abs().max()), float(w.abs().max()))
+
+
+def run_camera_sampling(device, points):
+    """the camera features at the points as one weighted lookup against eight gathers: the same products added in the same order, and the maps' gradient
+    against float64"""
+    from lidarseg3d_amd import point_heads
+    gen = torch.Generator().manual_seed(6)
+    img = tensor(gen, 2, 3, 48, 9, 13, device=device).requires_grad_()
+    cuv = torch.cat([torch.ones(points, 1), torch.randint(0, 3, (points, 1), generator=gen).float() - 1.0, torch.rand(points, 2, generator=gen) * 2.4 - 1.2], 1).to(device)
+    bidx = (torch.arange(points) * 2 // points).float().to(device)
+    want, got = point_heads._sample_image_rows(img, cuv, bidx), point_heads._sample_image_rows(img, cuv, bidx, lookup=True)
+    check(got, want.detach().cpu().double(), got.detach().cpu().double().abs().amax(1, keepdim=True) + 1.0, what="sampled features")
+    dy = tensor(gen, points, 48, device=device)
+    (g,) = torch.autograd.grad(got, [img], [dy])
+    i64 = img.detach().cpu().double().requires_grad_()
+    w64 = point_heads._sample_image_rows(i64, cuv.cpu(), bidx.cpu())
+    (ref,) = torch.autograd.grad(w64, [i64], [dy.cpu().double()])
+    (mag,) = torch.autograd.grad(point_heads._sample_image_rows(i64, cuv.cpu(), bidx.cpu()), [i64], [dy.cpu().double().abs()])
+    check(g, ref, mag, what="d maps", k=(points + 16) * 2.0 ** -24)
+
+
+def run_use_in_training(device):
+    """use_in_training reaches the decoder, the reader and the heads' dropout, keeps the parameters' names, and state None undoes it"""
+    from lidarseg3d_amd import blocks, build_detector, models_cfg
+    model = build_detector(models_cfg.mseg3d(), train_cfg=None, test_cfg={}).to(device).train()
+    names = list(model.state_dict())
+    state = blocks.DropoutState(1, device=device)
+    assert blocks.use_in_training(model, state) is model
+    assert list(model.state_dict()) == names and model.point_head.block_state is state and model.point_head.sffm.block_state is state
+    drops = [m for m in model.modules() if isinstance(m, torch.nn.Dropout)]
+    assert drops and all(type(m) is blocks.Dropout and m.state is state and m.training for m in drops)
+    x = torch.ones(40, 32, device=device)
+    y = drops[0](x)
+    assert state.calls == 1 and 0 < int((y == 0).sum()) < y.numel() and torch.equal(drops[0].eval()(x), x)
+    blocks.use_in_training(model, None)
+    assert model.point_head.block_state is None and all(m.state is None for m in drops)

@@ -49,6 +49,23 @@ def test_a_block_of_all_three_operators(rows, width, table):
     bc.run_block(DEV, rows, width, table)
 
 
+@pytest.mark.parametrize("points,p", [(300, 0.0), (300, 0.1), (70000, 0.1)])
+def test_decoder_training_forward(points, p, monkeypatch):
+    bc.run_decoder(DEV, points, p, monkeypatch)
+
+
+def test_reader_training_forward():
+    bc.run_reader(DEV, 5000)
+
+
+def test_camera_sampling():
+    bc.run_camera_sampling(DEV, 6000)
+
+
+def test_use_in_training():
+    bc.run_use_in_training(DEV)
+
+
 def test_dropout_rate_and_independence_of_calls():
     """2^22 draws at p = 0.1: the share that is dropped is within 6 standard deviations, and two calls agree in p^2 + (1 - p)^2 of the places"""
     from lidarseg3d_amd import blocks

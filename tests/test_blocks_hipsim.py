@@ -68,6 +68,25 @@ def test_masked_rows_and_values():
     bc.run_masked_rows("cpu")
 
 
+@pytest.mark.parametrize("p", [0.0, 0.1])
+def test_decoder_training_forward(p, monkeypatch):
+    bc.run_decoder("cpu", 23, p, monkeypatch)
+
+
+def test_reader_training_forward():
+    bc.run_reader("cpu", 11)
+
+
+def test_camera_sampling():
+    bc.run_camera_sampling("cpu", 60)
+
+
+def test_use_in_training():
+    bc.run_use_in_training("cpu")
+    with pytest.raises(TypeError, match="DropoutState"):
+        blocks.use_in_training(torch.nn.Linear(2, 2), torch.zeros(2, dtype=torch.int64))
+
+
 def test_refusals():
     x, st = torch.randn(4, 8), blocks.DropoutState(1, device="cpu")
     N = blocks.Norm("layer", torch.ones(8), torch.zeros(8))

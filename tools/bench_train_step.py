@@ -29,6 +29,10 @@ def main():
     ap.add_argument("--syncbn", action="store_true", help="BatchNorm1d -> CountSyncBatchNorm1d (statistics over all ranks, weighted by row counts)")
     ap.add_argument("--ddp", action="store_true", help="wrap the model in DistributedDataParallel (RCCL gradient all-reduce); "
                     "launch with python -m torch.distributed.run --nproc-per-node N --master-addr 127.0.0.1 ... (N = 1 works too)")
+    ap.add_argument("--block-operators", action="store_true", help="blocks.use_in_training: the transformer blocks' residual / dropout / norm in one pass each, "
+                    "counter-based dropout, the camera sampling as one weighted lookup")
+    ap.add_argument("--decoder-dropout", type=float, default=None, help="dropout of the SF-Phase decoder (the shipped configs: 0)")
+    ap.add_argument("--image-grad", action="store_true", help="gradients for the camera maps too, as a step that trains the camera network needs them")
     ap.add_argument("--profile-ops", type=int, default=0, help="print the N most expensive torch ops of one step with their input shapes and exit")
     args = ap.parse_args()
     import lidarseg3d_amd as L
@@ -41,7 +45,14 @@ def main():
     torch.manual_seed(0)
     ops.set_precision(args.precision)
     mcfg = getattr(models_cfg, args.model)(num_class=ncls, pc_range=cfg["pc_range"], voxel_size=cfg["voxel_size"])
+    if args.decoder_dropout is not None:
+        mcfg["point_head"]["model_cfg"]["SFPhase_CFG"]["drop_ratio"] = args.decoder_dropout
     model = L.build_detector(mcfg, train_cfg=None, test_cfg={})
+    state = None
+    if args.block_operators:
+        from lidarseg3d_amd import blocks
+        state = blocks.DropoutState(rank, device=dev)
+        blocks.use_in_training(model, state)
     if args.syncbn:
         from lidarseg3d_amd import syncbn
         model = syncbn.convert_sync_batchnorm(model)
@@ -67,7 +78,7 @@ def main():
               voxel_sem_labels=torch.randint(0, ncls, (V,), device=dev), point_sem_labels=torch.randint(0, ncls, (pts.shape[0],), device=dev))
     if args.model == "mseg3d":  # camera CNN outputs at the shipped configs' shapes (6 / 5 cameras, 48 channels, 160x240 maps)
         img, emb, cuv = synth.camera_inputs(pts.shape[0], seed=rank, ncam=ncam, c_img=48, h=160, w=240, num_class=ncls, batch=B)
-        ex.update(image_features=torch.from_numpy(img).to(dev), camera_semantic_embeddings=torch.from_numpy(emb).to(dev),
+        ex.update(image_features=torch.from_numpy(img).to(dev).requires_grad_(args.image_grad), camera_semantic_embeddings=torch.from_numpy(emb).to(dev),
                   points_cuv=torch.from_numpy(cuv).to(dev))
     opt = torch.optim.SGD(model.parameters(), lr=0.01, momentum=0.9)
     if args.profile_ops:  # which torch ops (with input shapes) the step spends its GPU time in: what is left on torch autograd
@@ -93,6 +104,8 @@ def main():
         loss.backward()
         torch.cuda.synchronize(); t2 = time.perf_counter()
         opt.step()
+        if state is not None:
+            state.advance()
         torch.cuda.synchronize(); t3 = time.perf_counter()
         losses.append(float(loss.detach()))
         if it >= args.warmup:
@@ -105,7 +118,9 @@ def main():
         dist.destroy_process_group()
     if rank == 0:
         print(json.dumps({"what": args.model + " training step (" + args.precision + "), %s geometry, %d frame(s) per GPU, %d GPU(s)%s%s"
-                                  % (args.geometry, B, world, ", DDP" if args.ddp else "", ", count-weighted SyncBN" if args.syncbn else ""),
+                                  % (args.geometry, B, world, ", DDP" if args.ddp else "", ", count-weighted SyncBN" if args.syncbn else "")
+                                  + (", block operators" if state is not None else "") + (", gradients for the camera maps" if args.image_grad else "")
+                                  + (", decoder dropout %g" % args.decoder_dropout if args.decoder_dropout is not None else ""),
                           "points_per_frame": args.points, "frames_per_gpu": B, "active_voxels": V,
                           "forward_ms": 1e3 * tf / k, "backward_ms": 1e3 * tb / k, "optimizer_ms": 1e3 * to / k,
                           "step_ms": 1e3 * (tf + tb + to) / k, "frames_per_s": world * B * k / (tf + tb + to),
