@@ -115,15 +115,6 @@ def _configure(lib):
                  "ls3d_dynamic_point_to_voxel_workspace_bytes", "ls3d_unique_sorted_workspace_bytes",
                  "ls3d_residual_norm_workspace_bytes", "ls3d_embedding_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
-    # the training-block operators are called with plain integers (an argument object each would be a third of a small call's host time)
-    P, ll, i, f, u, z = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_uint32, ctypes.c_size_t
-    D = ctypes.POINTER(ResidualNorm)
-    for name, types in (("ls3d_dropout_forward", (P, ll, ll, ll, i, f, P, u, i, P, P, P)), ("ls3d_dropout_backward", (P, ll, P, ll, ll, i, f, P, u, i, P, P)),
-                        ("ls3d_residual_norm_forward", (P, ll, P, ll, i, i, D, P, P, P, P)), ("ls3d_residual_norm_workspace_bytes", (i, i)),
-                        ("ls3d_residual_norm_backward", (P, ll, P, ll, i, i, D, P, P, ll, P, ll, P, P, P, P, P, P, P, P, z, P)),
-                        ("ls3d_embedding_forward", (P, ll, ll, i, i, P, i, i, i, P, f, P, P)), ("ls3d_embedding_workspace_bytes", (i, i, i)),
-                        ("ls3d_embedding_backward", (P, ll, ll, i, i, P, i, i, i, P, f, ll, P, ll, P, P, P, z, P))):
-        getattr(lib, name).argtypes = types
     for name in EXPORTS:
         fn = getattr(lib, name)  # AttributeError here = header/library mismatch: fail loudly
         if fn.restype is ctypes.c_int:
@@ -152,6 +143,27 @@ def use_library_for_testing(path):
     global _lib
     _lib = _configure(ctypes.CDLL(path)) if path else None
     return _lib
+
+
+_host = None
+_host_bound = None
+
+
+def host_module():
+    """the C++ side of blocks.py (csrc/host/blocks_autograd.cpp), its calls bound to the library in use"""
+    global _host, _host_bound
+    lib = load()
+    if _host_bound is not lib:
+        if _host is None:
+            try:
+                import torch  # noqa: F401  (the module links against it)
+                from . import _blocks_host
+            except ImportError as e:
+                raise LibraryMissing("lidarseg3d_amd/_blocks_host.so cannot be loaded (%s): build it with `python -m lidarseg3d_amd.build`" % e)
+            _host = _blocks_host
+        _host.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTS})
+        _host_bound = lib
+    return _host
 
 
 def check(rc, what):

@@ -15,9 +15,10 @@ camera sampling with a deterministic gradient)."""
 import torch
 from torch import nn
 
-from . import ops
+from . import _lib, ops
 
 _KINDS = {"layer": 1, "rms": 2}
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 class Norm(object):
@@ -71,33 +72,13 @@ class DropoutState(object):
 
 
 def _dtype_ok(t, what):
-    if t.dtype not in ops.DTYPES:
+    if t.dtype not in _TYPES:
         raise TypeError("%s: float32, bfloat16 or float16 needed, got %s" % (what, t.dtype))
 
 
 def _on_device(t, what):
     if not (t.is_cuda or ops._SIM):
         raise RuntimeError("%s: lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % (what, t.device))
-
-
-def _rows(t, c):
-    """t [..., c] as rows the kernels take: a view where the rows are contiguous, else a copy"""
-    r = t if t.dim() == 2 else t.reshape(-1, c) if c else t.reshape(0, 0)
-    if r.is_contiguous():
-        return r
-    if (c > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < c):
-        r = r.contiguous()
-    return r
-
-
-def _shaped(t, shape):
-    return t if t.shape == shape else t.reshape(shape)
-
-
-def _once(what):
-    """a second derivative would come out as a constant: refuse it (the check of torch's once_differentiable at a tenth of its cost)"""
-    if torch.is_grad_enabled():
-        raise RuntimeError("%s is differentiable once (backward with create_graph=True)" % what)
 
 
 def _draw(p, state, call):
@@ -120,22 +101,6 @@ def _draw(p, state, call):
 
 
 # ---------------------------------------------------------------------------------------------- dropout
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, state, call, relu):
-        y, bits = ops.dropout_forward(_rows(x, x.shape[-1]), p, state, call, relu, ctx.needs_input_grad[0])
-        ctx.save_for_backward(state, bits)
-        ctx.args = (p, call, relu)
-        return _shaped(y, x.shape)
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("dropout")
-        state, bits = ctx.saved_tensors
-        p, call, relu = ctx.args
-        return _shaped(ops.dropout_backward(_rows(dy, dy.shape[-1]), bits, p, state, call, relu), dy.shape), None, None, None, None
-
-
 def dropout(x, p, state, call=None, relu=False):
     """dropout(x) - relu: dropout(relu(x)) - over the last dimension's rows, the mask made from (seed, step, call, row, column) in the forward pass and
     again in the backward pass: it is never stored (relu: one bit per element says where x was positive and kept).
@@ -150,7 +115,7 @@ def dropout(x, p, state, call=None, relu=False):
         return dropout(x.reshape(1), p, state, call, relu).reshape(())
     if x.numel() == 0:
         return x
-    return _Dropout.apply(x, p, state, call, bool(relu))
+    return _lib.host_module().dropout(x, p, state, call, bool(relu))
 
 
 class Dropout(nn.Dropout):
@@ -167,38 +132,6 @@ class Dropout(nn.Dropout):
 
 
 # ---------------------------------------------------------------------------------------------- residual, dropout, gate and norms
-class _ResidualNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, gate, w_in, b_in, w_out, b_out, state, cfg):
-        kind_in, eps_in, kind_out, eps_out, alpha, p, call, want_sum = cfg
-        norms = ((kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None)
-        y, s, stats = ops.residual_norm_forward(x, residual, gate, norms[0], norms[1], alpha, p, state, call, want_sum)
-        ctx.save_for_backward(x, residual, gate, w_in, b_in, w_out, b_out, state, stats)
-        ctx.cfg = cfg
-        ctx.set_materialize_grads(False)
-        return (y, s) if kind_out and want_sum else (y if kind_out else s)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        _once("residual_norm")
-        x, residual, gate, w_in, b_in, w_out, b_out, state, stats = ctx.saved_tensors
-        kind_in, eps_in, kind_out, eps_out, alpha, p, call, want_sum = ctx.cfg
-        dy, ds = (grads if len(grads) == 2 else (grads[0], None)) if kind_out else (None, grads[0])
-        if dy is None and ds is None:
-            return (None,) * 9
-        c = x.shape[1]
-        want = list(ctx.needs_input_grad[:7])
-        # s = residual + x: one gradient for both, written once
-        same = want[0] and want[1] and residual is not None and gate is None and not kind_in and p == 0.0 and alpha == 1.0 and x.dtype == residual.dtype
-        if same:
-            want[0] = False
-        out = ops.residual_norm_backward(x, residual, gate, (kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None,
-                                         alpha, p, state, call, stats, None if dy is None else _rows(dy, c), None if ds is None else _rows(ds, c), want)
-        if same:
-            out[0] = out[1]
-        return (*out, None, None)
-
-
 def _norm_arguments(nm, c, what):
     """-> weight, bias, kind, eps of a Norm or None, checked against rows of c values"""
     if nm is None:
@@ -208,7 +141,7 @@ def _norm_arguments(nm, c, what):
     out = []
     for t in (nm.weight, nm.bias):
         if t is not None:
-            if t.dtype not in ops.DTYPES:
+            if t.dtype not in _TYPES:
                 _dtype_ok(t, what + " parameter")
             if t.dim() != 1 or t.shape[0] != c:
                 raise ValueError("%s: weight and bias of shape [%d] needed, got %s" % (what, c, tuple(t.shape)))
@@ -242,7 +175,6 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
         if gate.shape == shape and gate.dim() > 1:
             if gate.dtype != x.dtype:
                 raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
-            gate = _rows(gate, c)
         elif gate.numel() == 1 or gate.shape == (c,):
             gate = gate if gate.shape == (c,) else gate.reshape(1).expand(c)
             if not gate.is_contiguous():
@@ -252,34 +184,11 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
     w_in, b_in, kind_in, eps_in = _norm_arguments(norm_in, c, "norm_in")
     w_out, b_out, kind_out, eps_out = _norm_arguments(norm, c, "norm")
     p, state, call = _draw(p, state, call)
-    x2, r2 = _rows(x, c), None if residual is None else _rows(residual, c)
-    alpha, return_sum = float(alpha), bool(return_sum)
-    if torch.is_grad_enabled() and (x2.requires_grad or any(t is not None and t.requires_grad for t in (r2, gate, w_in, b_in, w_out, b_out))):
-        res = _ResidualNorm.apply(x2, r2, gate, w_in, b_in, w_out, b_out, state, (kind_in, eps_in, kind_out, eps_out, alpha, p, call, return_sum))
-    else:
-        y, s, _ = ops.residual_norm_forward(x2, r2, gate, (kind_in, w_in, b_in, eps_in) if kind_in else None, (kind_out, w_out, b_out, eps_out) if kind_out else None,
-                                            alpha, p, state, call, return_sum, want_stats=False)
-        res = (y, s) if kind_out and return_sum else (y if kind_out else s)
-    return tuple(_shaped(t, shape) for t in res) if isinstance(res, tuple) else _shaped(res, shape)
+    out = _lib.host_module().residual_norm(x, residual, gate, w_in, b_in, w_out, b_out, state, kind_in, eps_in, kind_out, eps_out, float(alpha), p, call, bool(return_sum))
+    return tuple(out) if len(out) == 2 else out[0]
 
 
 # ---------------------------------------------------------------------------------------------- row lookup
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, weight, idx, scale, padding):
-        ctx.save_for_backward(table, weight, idx)
-        ctx.args = (scale, padding)
-        return ops.embedding_forward(table, idx, weight, scale)
-
-    @staticmethod
-    def backward(ctx, dout):
-        _once("embedding")
-        table, weight, idx = ctx.saved_tensors
-        scale, padding = ctx.args
-        dt, dw = ops.embedding_backward(table, idx, weight, scale, padding, _rows(dout, dout.shape[-1]), ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return dt, dw, None, None, None
-
-
 def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
     """scale * table[idx] of a table [rows, c]; idx int32 / int64 of any shape.  bag: the sum over idx's last dimension [..., k], with `weight` (float32, idx's
     shape) the weighted sum, scale * sum_j weight[..., j] * table[idx[..., j]].  An index outside [0, rows) - -1 by custom - names no row: it reads as zero and takes no
@@ -303,11 +212,11 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
         raise ValueError("padding_idx %r outside a table of %d rows" % (padding_idx, table.shape[0]))
     padding = -1 if padding_idx is None else int(padding_idx) % table.shape[0]
     lead, k = (idx.shape[:-1], idx.shape[-1]) if bag else (idx.shape, 1)
-    flat, tab, wgt = idx.reshape(-1, k).contiguous(), _rows(table, table.shape[1]), None if weight is None else weight.reshape(-1, k).contiguous()
-    if torch.is_grad_enabled() and (tab.requires_grad or (wgt is not None and wgt.requires_grad)):
-        out = _Embedding.apply(tab, wgt, flat, float(scale), padding)
-    else:
-        out = ops.embedding_forward(tab, flat, wgt, float(scale))
+    if idx.dim() != 2 or not bag or not idx.is_contiguous():
+        idx = idx.reshape(-1, k).contiguous()
+    if weight is not None and (weight.dim() != 2 or not weight.is_contiguous()):
+        weight = weight.reshape(-1, k).contiguous()
+    out = _lib.host_module().embedding(table, weight, idx, float(scale), padding)
     return out if len(lead) == 1 else out.reshape(*lead, table.shape[1])
 
 

@@ -3,7 +3,7 @@
     python -m lidarseg3d_amd.build            # build what is stale
     python -m lidarseg3d_amd.build --force
 
-Every csrc/*.hip is compiled to its own object (in parallel, only when it or a header changed) and the objects are
+csrc/host/blocks_autograd.cpp (the autograd side of blocks.py) becomes lidarseg3d_amd/_blocks_host.so.  Every csrc/*.hip is compiled to its own object (in parallel, only when it or a header changed) and the objects are
 linked into lidarseg3d_amd/libls3d.so.  hipcc cross-compiles without a GPU, so this also runs in the CPU-only
 development container (__graft_entry__.build()).  The built .so is git-ignored but travels to the GPU box with the
 snapshot; the objects live in lidarseg3d_amd/_obj/ (git- and gpurun-ignored).
@@ -31,6 +31,29 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")))
 
 
+HOST_SRC = os.path.join(CSRC, "host", "blocks_autograd.cpp")
+HOST_LIB = os.path.join(HERE, "_blocks_host.so")
+
+
+def build_host(force=False, verbose=False):
+    """the autograd side of blocks.py: plain C++ against torch's headers, no device code"""
+    if not force and not _stale(HOST_LIB, [HOST_SRC, os.path.join(HERE, "..", "include", "ls3d.h")]):
+        return HOST_LIB
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-w", "-DTORCH_EXTENSION_NAME=_blocks_host", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += ["-I" + d for d in inc] + [HOST_SRC, "-L" + os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-o", HOST_LIB + ".tmp"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)  # a process that has the old one loaded keeps it
+    return HOST_LIB
+
+
 def _headers():
     return glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(HERE, "..", "include", "ls3d.h")]
 
@@ -47,7 +70,7 @@ def _stale(target, deps):
 
 
 def is_stale():
-    return _stale(LIB, sources() + _headers())
+    return _stale(LIB, sources() + _headers()) or _stale(HOST_LIB, [HOST_SRC, os.path.join(HERE, "..", "include", "ls3d.h")])
 
 
 def build(force=False, verbose=False):
@@ -64,8 +87,10 @@ def build(force=False, verbose=False):
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
 
-    with ThreadPoolExecutor(max_workers=min(8, max(1, len(todo)))) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, 1 + len(todo))) as ex:
+        host = ex.submit(build_host, force, verbose)
         list(ex.map(cc, todo))
+        host.result()
     cmd = [hipcc, "-shared", "-fPIC", "--offload-arch=" + ARCH, "-fno-gpu-rdc"] + [_obj(s) for s in sources()] + ["-o", LIB]
     if verbose:
         print(" ".join(cmd), flush=True)

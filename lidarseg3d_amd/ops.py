@@ -1832,151 +1832,3 @@ def batch_norm_train(bn, x, res=None, relu=False):
             bn.running_mean.mul_(1 - m).add_(mean, alpha=m)
             bn.running_var.mul_(1 - m).add_(var * (count / (count - 1.0).clamp_min(1.0)), alpha=m)  # unbiased, as nn.BatchNorm does
     return y
-
-
-# ---------------------------------------------------------------------------------------------- training-block operators (lidarseg3d_amd/blocks.py)
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # LS3D_DTYPE_*
-
-
-def _row_view(t, name):
-    """(pointer, row stride) of a 2-D tensor whose rows are contiguous; any row stride from the row's length on"""
-    if t is None:
-        return None, 0
-    (n, c), (ld, unit) = t.shape, t.stride()
-    if (c > 1 and unit != 1) or (n > 1 and ld < c):
-        raise RuntimeError("%s: 2-D tensor with contiguous rows needed (shape %s, strides %s)" % (name, tuple(t.shape), t.stride()))
-    if t.is_cuda == _SIM:
-        _wrong_device(t)
-    return t.data_ptr(), ld if n > 1 else (c or 1)
-
-
-def _wrong_device(t):
-    raise RuntimeError("hipsim test hook active: CPU tensors only" if _SIM else
-                       "lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % t.device)
-
-
-def _addr(t):
-    """data pointer of a contiguous tensor (None stays None) as a plain integer, for the entry points whose argument types _lib declares"""
-    if t is None:
-        return None
-    if not t.is_contiguous():
-        raise RuntimeError("non-contiguous tensor passed to libls3d")
-    if t.is_cuda == _SIM:
-        _wrong_device(t)
-    return t.data_ptr()
-
-
-def _same_device(ref, *others):
-    dev = ref.device
-    for t in others:
-        if t is not None and t.device != dev:
-            raise RuntimeError("tensors on different devices: %s and %s" % (dev, t.device))
-
-
-def _call_on(t, fn, what, *args):
-    """the C call with the tensor's device current (a launch on another device's stream would fail) and on its current stream"""
-    dev = t.get_device()
-    if dev < 0:
-        rc = fn(*args, None)
-    elif dev == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        check(rc, what)
-
-
-def _fresh(t):
-    """a new contiguous tensor of t's shape, type and device"""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def dropout_forward(x, p, state, call, relu=False, want_bits=False):
-    """x [rows, c] (contiguous rows) -> (y of its type, bits): ls3d_dropout_forward; state: int64 [2] (seed, step) on the device.  bits (relu and
-    want_bits, else None): uint8 [rows, ceil(c / 8)], what dropout_backward needs to know of x"""
-    _same_device(x, state)
-    y = _fresh(x)
-    bits = torch.empty((x.shape[0], (x.shape[1] + 7) // 8), dtype=torch.uint8, device=x.device) if relu and want_bits else None
-    px, ld = _row_view(x, "x")
-    _call_on(x, _L().ls3d_dropout_forward, "ls3d_dropout_forward", px, ld, x.shape[0], x.shape[1], DTYPES[x.dtype], p, _addr(state), call, int(relu), _addr(y), _addr(bits))
-    return y, bits
-
-
-def dropout_backward(dy, bits, p, state, call, relu=False):
-    """dx from dy [rows, c] and - relu - the forward's bits (ls3d_dropout_backward)"""
-    dx = _fresh(dy)
-    pd, ld = _row_view(dy, "dy")
-    _call_on(dy, _L().ls3d_dropout_backward, "ls3d_dropout_backward", pd, ld, _addr(bits), dy.shape[0], dy.shape[1], DTYPES[dy.dtype], p, _addr(state), call, int(relu),
-             _addr(dx))
-    return dx
-
-
-def residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call):
-    """ls3d_residual_norm_t; norm_in / norm_out: None or (kind 1 layer | 2 rms, weight, bias, eps); gate: None, [c] or [n, c]"""
-    norms = [_lib.Norm() if nm is None else
-             _lib.Norm(_addr(nm[1]), _addr(nm[2]), nm[0], 0 if nm[1] is None else DTYPES[nm[1].dtype], 0 if nm[2] is None else DTYPES[nm[2].dtype], nm[3])
-             for nm in (norm_in, norm_out)]
-    kind, g, ld, gt = 0, None, 0, 0
-    if gate is not None:
-        gt = DTYPES[gate.dtype]
-        if gate.dim() == 1:
-            kind, g = 1, _addr(gate)
-        else:
-            kind, (g, ld) = 2, _row_view(gate, "gate")
-    dt = DTYPES[x.dtype]
-    return _lib.ResidualNorm(norms[0], norms[1], g, ld, _addr(state), dt, dt if residual is None else DTYPES[residual.dtype], kind, gt, alpha, p, call)
-
-
-def residual_norm_forward(x, residual=None, gate=None, norm_in=None, norm_out=None, alpha=1.0, p=0.0, state=None, call=0, want_sum=False, want_stats=True):
-    """-> (y or None, s or None, stats [n, 4] or None) of ls3d_residual_norm_forward; x [n, c], residual [n, c] (of x's type or f32)"""
-    n, c = x.shape
-    _same_device(x, residual, gate, state, *[t for nm in (norm_in, norm_out) if nm is not None for t in nm[1:3]])
-    d = residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call)
-    y = _fresh(x) if norm_out is not None else None
-    s = _fresh(x if residual is None else residual) if want_sum or norm_out is None else None
-    stats = torch.empty((n, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    px, x_ld = _row_view(x, "x")
-    pr, r_ld = _row_view(residual, "residual")
-    _call_on(x, _L().ls3d_residual_norm_forward, "ls3d_residual_norm_forward", px, x_ld, pr, r_ld, n, c, ctypes.byref(d),
-             _addr(y), _addr(s), _addr(stats))
-    return y, s, stats
-
-
-def residual_norm_backward(x, residual, gate, norm_in, norm_out, alpha, p, state, call, stats, dy, ds, want):
-    """gradients (x, residual, gate, in weight, in bias, out weight, out bias) - None where `want` (7 truth values) says so - of residual_norm_forward
-    (ls3d_residual_norm_backward); dy / ds: the gradients of y and s, None where that output was not used"""
-    n, c = x.shape
-    d = residual_norm_desc(x, residual, gate, norm_in, norm_out, alpha, p, state, call)
-    like = (x, residual, gate) + (norm_in[1:3] if norm_in is not None else (None, None)) + (norm_out[1:3] if norm_out is not None else (None, None))
-    grads = [_fresh(t) if w and t is not None else None for t, w in zip(like, want)]
-    L = _L()
-    ws = _ws(L.ls3d_residual_norm_workspace_bytes(n, c), x)
-    (px, x_ld), (pr, r_ld), (py, y_ld), (ps, s_ld) = _row_view(x, "x"), _row_view(residual, "residual"), _row_view(dy, "dy"), _row_view(ds, "ds")
-    _call_on(x, L.ls3d_residual_norm_backward, "ls3d_residual_norm_backward", px, x_ld, pr, r_ld, n, c, ctypes.byref(d), _addr(stats), py, y_ld, ps, s_ld,
-             *[_addr(g) for g in grads], _addr(ws), ws.numel())
-    return grads
-
-
-def embedding_forward(table, idx, weight=None, scale=1.0):
-    """scale * sum_j weight[i, j] * table[idx[i, j]]: table [rows, c], idx [n, k] int32 / int64, weight [n, k] f32 -> [n, c] (ls3d_embedding_forward)"""
-    _same_device(table, idx, weight)
-    (n, k), c = idx.shape, table.shape[1]
-    out = torch.empty((n, c), dtype=table.dtype, device=table.device)
-    pt, ld = _row_view(table, "table")
-    _call_on(table, _L().ls3d_embedding_forward, "ls3d_embedding_forward", pt, ld, table.shape[0], c, DTYPES[table.dtype], _addr(idx),
-             int(idx.dtype == torch.int64), n, k, _addr(weight), scale, _addr(out))
-    return out
-
-
-def embedding_backward(table, idx, weight, scale, padding, dout, want_table=True, want_weight=False):
-    """(gradient of the table, gradient of the weights) of embedding_forward, None where not wanted (ls3d_embedding_backward)"""
-    (n, k), (rows, c) = idx.shape, table.shape
-    dt = _fresh(table) if want_table else None
-    dw = torch.empty((n, k), dtype=torch.float32, device=table.device) if want_weight else None
-    L = _L()
-    ws = _ws(L.ls3d_embedding_workspace_bytes(n, k, c), table)
-    (pt, ld), (po, o_ld) = _row_view(table, "table"), _row_view(dout, "dout")
-    _call_on(table, L.ls3d_embedding_backward, "ls3d_embedding_backward", pt, ld, rows, c, DTYPES[table.dtype], _addr(idx), int(idx.dtype == torch.int64), n, k,
-             _addr(weight), scale, padding, po, o_ld, _addr(dt), _addr(dw), _addr(ws), ws.numel())
-    return dt, dw

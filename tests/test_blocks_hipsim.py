@@ -16,6 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 def sim_library():
     sys.path.insert(0, os.path.join(HERE, "hipsim"))
     import build_sim
+    from lidarseg3d_amd import build
+    build.build_host()  # (only where it is missing or older than its source)
     _lib.use_library_for_testing(build_sim.build())
     ops.set_sim(True)
     yield
@@ -146,6 +148,10 @@ def test_refusals():
     st.advance()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+    # second derivatives are refused, not answered as if the first were constant
+    for y, leaf in ((blocks.dropout(x, 0.5, st), x), (blocks.residual_norm(x, norm=N), x), (blocks.embedding(x, torch.zeros(3, dtype=torch.int64)), x)):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y.sum(), [leaf], create_graph=True)
     ops.set_sim(False)
     try:
         with pytest.raises(RuntimeError, match="no CPU fallback"):
