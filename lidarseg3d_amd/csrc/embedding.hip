@@ -18,7 +18,8 @@ __device__ __forceinline__ long long emb_index(const void *__restrict__ idx, int
 }
 
 // One chunk of 8 columns of one output row per thread; I: 32 bits where the chunk count allows.  A lookup is a chain of two round trips (index, table row), so
-// several are kept in flight: U entries of a row that sums k > 1 of them, U rows of one entry each (grid-stride apart) for k = 1.
+// U entries of a row that sums several are kept in flight.  (k = 1: four rows a thread in flight on 2048 workgroups or one on up to 16384 make no difference,
+// 360000 x 64 f32 26.5 / 24.8 us.)
 template <typename T, typename I, int U>
 __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total, int k,
                                                  const float *__restrict__ weight, float scale, T *__restrict__ out) {
@@ -57,43 +58,6 @@ __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, si
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] *= scale;
     ls3d_store8<T>(out + (size_t)i * c + col, acc, m);
-  }
-}
-
-template <typename T, typename I, int U>
-__global__ __launch_bounds__(256) void k_emb_fwd_one(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total,
-                                                     const float *__restrict__ weight, float scale, T *__restrict__ out) {
-  const uint32_t groups = (uint32_t)(c + 7) / 8;
-  const I step = (I)gridDim.x * 256;
-  for (I t0 = (I)blockIdx.x * 256 + threadIdx.x; t0 < total; t0 += step * U) {
-    uint32_t i[U], g[U];
-    long long v[U];
-    float w[U];
-    ls3d_raw8<T> r[U];
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const I t = t0 + step * q < total ? t0 + step * q : t0;
-      i[q] = (uint32_t)(t / groups);
-      g[q] = (uint32_t)(t - (I)i[q] * groups);
-      v[q] = emb_index(idx, is64, i[q]);
-      w[q] = (weight ? weight[i[q]] : 1.0f) * scale;
-    }
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      r[q] = ls3d_raw8<T>{};
-      if (v[q] >= 0 && v[q] < rows) r[q] = ls3d_load8<T>(table + (size_t)v[q] * table_ld, (long long)g[q] * 8, c);
-    }
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      if (q > 0 && t0 + step * q >= total) break;
-      const int col = (int)g[q] * 8, m = c - col;
-      float x[8];
-      ls3d_unpack8<T>(r[q], m, x);
-      const bool hit = v[q] >= 0 && v[q] < rows;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = hit ? x[j] * w[q] : 0.0f;  // (a weight of NaN beside an index that names no row is not seen)
-      ls3d_store8<T>(out + (size_t)i[q] * c + col, x, m);
-    }
   }
 }
 
@@ -403,26 +367,26 @@ __global__ __launch_bounds__(256) void k_emb_tiles(const uint2 *__restrict__ pai
 // The long rows: partial[j][1] + partial[j + 1][0] + ... from the tile j in which the row begins, while the tiles begin with it.  A workgroup looks at EJ_TILES
 // tiles (few are such a j) and takes what it finds one after the other, all its threads together: `lpr` lanes per partial row, the 256 / lpr groups take the tiles in
 // turn (one wave walking the 700 tiles of a row one after the other took 210 us), their sums are added in order.
-constexpr int EJ_TILES = 16;
+constexpr int EJ_TILES = 16;  // at most; `span`: fewer where there are few tiles
 template <typename T>
-__global__ __launch_bounds__(256) void k_emb_join(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int lpr, int c, float scale,
+__global__ __launch_bounds__(256) void k_emb_join(const uint2 *__restrict__ pairs, const int32_t *__restrict__ n_valid, int tile, int span, int lpr, int c, float scale,
                                                   const float *__restrict__ partial, T *__restrict__ dtable) {
-  __shared__ float s_sum[256][9];
+  __shared__ float s_sum[4][64][9];
   __shared__ int s_begin[EJ_TILES], s_rest;
   const int N = *n_valid;
-  const long long j0 = (long long)blockIdx.x * EJ_TILES, mine = (j0 + threadIdx.x + 1) * tile;  // `mine`: where this thread's tile ends
+  const long long j0 = (long long)blockIdx.x * span, mine = (j0 + threadIdx.x + 1) * tile;  // `mine`: where this thread's tile ends
   if (j0 * tile >= N) return;
   bool begins = false;
-  if (threadIdx.x < EJ_TILES && mine + tile < N) {  // a long row that begins in the tile covers the next one and goes on (or ends) behind it
+  if ((int)threadIdx.x < span && mine + tile < N) {  // a long row that begins in the tile covers the next one and goes on (or ends) behind it
     const uint32_t row = pairs[mine - 1].x;
     begins = pairs[mine].x == row && pairs[mine + tile].x == row && !(mine > tile && pairs[mine - tile].x == row && pairs[mine - tile - 1].x == row);
   }
-  if (threadIdx.x < EJ_TILES) s_begin[threadIdx.x] = begins;
+  if ((int)threadIdx.x < span) s_begin[threadIdx.x] = begins;
   if (__syncthreads_count(begins) == 0) return;
   const int lane = (int)threadIdx.x % lpr, grp = (int)threadIdx.x / lpr, ngrp = 256 / lpr;
   const int col = ((int)blockIdx.y * lpr + lane) * 8, m = c - col;
   const int ntiles = (int)(((long long)N + tile - 1) / tile);
-  for (int q0 = 0; q0 < EJ_TILES; ++q0) {
+  for (int q0 = 0; q0 < span; ++q0) {
     if (!s_begin[q0]) continue;  // uniform
     const int j = (int)j0 + q0;
     const uint32_t cur = pairs[((long long)j + 1) * tile - 1].x;
@@ -454,16 +418,17 @@ __global__ __launch_bounds__(256) void k_emb_join(const uint2 *__restrict__ pair
         for (int q = 0; q < 8; ++q) acc[q] += p[q];
       }
     }
+    // the wave's groups by lane exchange, the four waves through LDS, in order
 #pragma unroll
-    for (int q = 0; q < 8; ++q) s_sum[threadIdx.x][q] = acc[q];
+    for (int q = 0; q < 8; ++q) {
+      for (int d = lpr; d < 64; d <<= 1) acc[q] += __shfl_xor(acc[q], d);
+      s_sum[threadIdx.x >> 6][threadIdx.x & 63][q] = acc[q];
+    }
     __syncthreads();
     if (grp == 0 && m > 0) {
       ls3d_unpack8<float>(ls3d_load8<float>(partial + ((size_t)j * 2 + 1) * c, col, c), m, acc);
-      for (int g = 0; g < ngrp; ++g)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += s_sum[g * lpr + lane][q];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] *= scale;
+      for (int q = 0; q < 8; ++q) acc[q] = (acc[q] + ((s_sum[0][lane][q] + s_sum[1][lane][q]) + (s_sum[2][lane][q] + s_sum[3][lane][q]))) * scale;
       ls3d_store8<T>(dtable + (size_t)cur * c + col, acc, m);
     }
     __syncthreads();
@@ -520,24 +485,20 @@ extern "C" int ls3d_embedding_forward(const void *table, long long table_ld, lon
   const long long total = (long long)n * ((c + 7) / 8);
   const int is64 = idx_dtype == LS3D_INDEX_I64;
 #define EMB_FWD(I_, U_)                                                                                                                                                   \
-  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, I_, U_>), ls3d_grid(total), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (I_)total, k, \
+  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, I_, U_>), ls3d_grid(total, 256, U_ == 1 ? 16384 : 2048), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (I_)total, k, \
                                       weight, scale, (T *)out))
-#define EMB_FWD_ONE(I_, U_)                                                                                                                                               \
-  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd_one<T, I_, U_>), ls3d_grid(total), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,         \
-                                      (I_)total, weight, scale, (T *)out))
   if (total < (1ll << 30)) {  // (the strides on top stay below 2^32)
-    if (k == 1) EMB_FWD_ONE(uint32_t, 4);
+    if (k == 1) EMB_FWD(uint32_t, 1);
     else if (k <= 4) EMB_FWD(uint32_t, 4);
     else EMB_FWD(uint32_t, 8);
-  } else if (k == 1) EMB_FWD_ONE(unsigned long long, 4);
-  else EMB_FWD(unsigned long long, 4);
+  } else EMB_FWD(unsigned long long, 4);
 #undef EMB_FWD
-#undef EMB_FWD_ONE
   LS3D_RETURN_IF_LAUNCH_FAILED();
   return LS3D_OK;
 }
 
-// entries per tile: the lanes of a large call fill the card four times over even if two thirds of its entries name no row; 8 to 64 entries
+// entries per tile: the lanes of a large call fill the card four times over even if two thirds of its entries name no row; 8 to 64 entries.  (360000 entries of 32
+// rows x 64 f32: 19 us in tiles of 16, 39 in tiles of 64, where the join has a quarter of the partial sums and is 5 us shorter.)
 static inline int emb_tile(long long entries, int c) {
   const long long want = entries * ((c + 7) / 8) / 262144;
   int t = 8;
@@ -630,8 +591,11 @@ static int emb_table_gradient(const emb_keys &K, int entries, int c, int k, cons
   const int32_t *n_valid = (const int32_t *)(ws + S.n_valid);
   float *partial = (float *)(ws + S.partial);
   hipLaunchKernelGGL((k_emb_tiles<T, 8>), grid, dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, k, weight, scale, dout, dout_ld, dtable, partial);
-  if (ntiles > 1)
-    hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)((ntiles + EJ_TILES - 1) / EJ_TILES), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, scale, (const float *)partial, dtable);
+  if (ntiles > 1) {  // (16384 tokens of text in 8-entry tiles: 14 us on 16 tiles a workgroup, where several frequent tokens meet in one)
+    const int span = ntiles <= 4096 ? 2 : EJ_TILES;
+    hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)((ntiles + span - 1) / span), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, span, lpr, c, scale, (const float *)partial,
+                       dtable);
+  }
   return LS3D_OK;
 }
 
