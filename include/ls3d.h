@@ -835,7 +835,8 @@ int ls3d_residual_norm_backward(const void *x, long long x_ld, const void *resid
 
 /* Row lookup: out[i] = scale * sum_j weight[i][j] * table[idx[i][j]], j < k (weight NULL: 1).  An index outside [0, rows) names no row.
  * backward: dtable[rows, c] (all of it is written; NULL: not wanted) from the entries sorted by row and added in input order, without the row `padding`
- * (-1: none); dweight[n, k] (NULL: not wanted; needs the table).  workspace: ls3d_embedding_workspace_bytes(n, k, c) bytes, 16-byte aligned.  n * k < 2^30. */
+ * (-1: none); dweight[n, k] (NULL: not wanted; needs the table).  workspace: ls3d_embedding_workspace_bytes(n, k, c) bytes, 16-byte aligned.  n * k < 2^30,
+ * c <= 2^24. */
 int ls3d_embedding_forward(const void *table, long long table_ld, long long rows, int c, int dtype, const void *idx, int idx_dtype, int n, int k,
                            const float *weight, float scale, void *out, ls3d_stream_t stream);
 size_t ls3d_embedding_workspace_bytes(int n, int k, int c);

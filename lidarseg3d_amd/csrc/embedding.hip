@@ -460,9 +460,10 @@ __global__ __launch_bounds__(256) void k_emb_dweight(const T *__restrict__ table
   }
 }
 
+constexpr int EMB_MAX_C = 1 << 24;  // (a grid has at most 65535 slabs of 512 columns)
 static int emb_check(const void *table, long long table_ld, long long rows, int c, int dtype, const void *idx, int idx_dtype, int n, int k, const float *weight) {
   if (rows < 0 || rows > 0x7FFFFFFEll || c < 0 || n < 0 || k < 1 || !ls3d_dtype_ok(dtype) || (idx_dtype != LS3D_INDEX_I32 && idx_dtype != LS3D_INDEX_I64)) return LS3D_ERR_ARG;
-  if ((long long)n * k > 0x3FFFFFFFll) return LS3D_ERR_UNSUPPORTED;
+  if ((long long)n * k > 0x3FFFFFFFll || c > EMB_MAX_C) return LS3D_ERR_UNSUPPORTED;
   if (n == 0 || c == 0) return LS3D_OK;
   if (!idx || ((uintptr_t)idx & (idx_dtype == LS3D_INDEX_I64 ? 7 : 3)) || ((uintptr_t)weight & 3)) return LS3D_ERR_ARG;
   if (rows && (!table || table_ld < c || ((uintptr_t)table & (ls3d_dtype_size(dtype) - 1)))) return LS3D_ERR_ARG;
@@ -532,16 +533,10 @@ extern "C" size_t ls3d_embedding_workspace_bytes(int n, int k, int c) {
 }
 
 template <typename T, int ITEMS>
-static bool emb_sort_small(const emb_keys &K, int entries, int bits, int32_t *n_valid, uint2 *out, T *dtable, size_t elems, hipStream_t stream) {
+static void emb_sort_small(const emb_keys &K, int entries, int bits, int32_t *n_valid, uint2 *out, T *dtable, size_t elems, hipStream_t stream) {
   const int lds = 1024 * ITEMS * (int)sizeof(uint2) + 16 * 256 * 4;
-  static bool attr_set[LS3D_MAX_DEVICES] = {};  // the opt-in to > 64 KB of dynamic LDS is per device
-  bool &set = attr_set[ls3d_device_slot()];
-  if (!set && lds > 65536) {
-    if (hipFuncSetAttribute((const void *)k_es_small<T, ITEMS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return false;
-    set = true;
-  }
+  static_assert(1024 * ITEMS * sizeof(uint2) + 16 * 256 * 4 <= 65536, "dynamic LDS without an opt-in");
   hipLaunchKernelGGL((k_es_small<T, ITEMS>), dim3(1 + ls3d_grid((long long)(elems / 8 + 1), 1024, 1024).x), dim3(1024), lds, stream, K, entries, bits, n_valid, out, dtable, elems);
-  return true;
 }
 
 // sorts the entries and clears the gradient table; -> the sorted pairs
@@ -552,9 +547,9 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
   int32_t *n_valid = (int32_t *)(ws + S.n_valid), *totals = (int32_t *)(ws + S.totals), *hist = (int32_t *)(ws + S.hist);
   uint2 *buf[2] = {(uint2 *)(ws + S.pairs[0]), (uint2 *)(ws + S.pairs[1])};
   if (entries <= ES_SMALL) {
-    const bool ok = entries <= 1024   ? emb_sort_small<T, 1>(K, entries, bits, n_valid, buf[0], dtable, elems, stream)
-                                      : emb_sort_small<T, 4>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
-    return ok ? buf[0] : nullptr;
+    if (entries <= 1024) emb_sort_small<T, 1>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
+    else emb_sort_small<T, 4>(K, entries, bits, n_valid, buf[0], dtable, elems, stream);
+    return buf[0];
   }
   const int passes = emb_passes(bits), per = (bits + passes - 1) / passes, ntiles = es_tiles(entries), digits = 1 << per, items = es_items(entries);
   const unsigned clear = ls3d_grid((long long)(elems / 8 + 1)).x;
@@ -579,11 +574,10 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
 }
 
 template <typename T>
-static int emb_table_gradient(const emb_keys &K, int entries, int c, int k, const float *weight, float scale, const T *dout, size_t dout_ld, T *dtable, char *ws, hipStream_t stream) {
+static void emb_table_gradient(const emb_keys &K, int entries, int c, int k, const float *weight, float scale, const T *dout, size_t dout_ld, T *dtable, char *ws, hipStream_t stream) {
   const size_t elems = (size_t)K.rows * c;
   const emb_space S = emb_layout(entries, c);
   const uint2 *pairs = emb_sort<T>(K, entries, S, ws, dtable, elems, stream);
-  if (!pairs) return LS3D_ERR_LAUNCH;
   const int groups = (c + 7) / 8, tile = emb_tile(entries, c), ntiles = (entries + tile - 1) / tile;
   int lpr = 1;
   while (lpr < groups && lpr < 64) lpr *= 2;
@@ -591,12 +585,11 @@ static int emb_table_gradient(const emb_keys &K, int entries, int c, int k, cons
   const int32_t *n_valid = (const int32_t *)(ws + S.n_valid);
   float *partial = (float *)(ws + S.partial);
   hipLaunchKernelGGL((k_emb_tiles<T, 8>), grid, dim3(256), 0, stream, pairs, n_valid, tile, lpr, c, k, weight, scale, dout, dout_ld, dtable, partial);
-  if (ntiles > 1) {  // (16384 tokens of text in 8-entry tiles: 14 us on 16 tiles a workgroup, where several frequent tokens meet in one)
+  if (ntiles > 1) {  // (16384 tokens of text in 8-entry tiles: 14 us on 16 tiles a workgroup, where several frequent tokens meet in one, 12 on 2)
     const int span = ntiles <= 4096 ? 2 : EJ_TILES;
     hipLaunchKernelGGL((k_emb_join<T>), dim3((unsigned)((ntiles + span - 1) / span), grid.y), dim3(256), 0, stream, pairs, n_valid, tile, span, lpr, c, scale, (const float *)partial,
                        dtable);
   }
-  return LS3D_OK;
 }
 
 template <typename T>
@@ -627,8 +620,7 @@ extern "C" int ls3d_embedding_backward(const void *table, long long table_ld, lo
   if (dtable && rows > 0 && c > 0) {
     const emb_keys K = {idx, is64, rows, padding};
     if (entries > 0) {
-      EMB_TYPES(dtype, rc = emb_table_gradient<T>(K, entries, c, k, weight, scale, (const T *)dout, (size_t)dout_ld, (T *)dtable, (char *)workspace, stream));
-      if (rc != LS3D_OK) return rc;
+      EMB_TYPES(dtype, emb_table_gradient<T>(K, entries, c, k, weight, scale, (const T *)dout, (size_t)dout_ld, (T *)dtable, (char *)workspace, stream));
     } else {
       const size_t elems = (size_t)rows * c;
       EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_clear<T>), ls3d_grid((long long)(elems / 8 + 1)), dim3(256), 0, stream, (T *)dtable, elems));

@@ -374,6 +374,43 @@ def run_strides_and_absent_parts(device):
     assert bool((on == 0).all()) and bool((torch.autograd.grad(on.sum(), [t0])[0] == 0).all())
 
 
+def run_partial_gradients(device):
+    """any subset of the inputs may want a gradient: each alone gives the bits it gives among all; one tensor as x and residual, as both norms' weight"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(21)
+    base = dict(x=tensor(gen, 7, 40, device=device), residual=tensor(gen, 7, 40, device=device), gate=tensor(gen, 40, device=device), wi=tensor(gen, 40, device=device),
+                bi=tensor(gen, 40, device=device), wo=tensor(gen, 40, device=device), bo=tensor(gen, 40, device=device))
+    dy, ds = tensor(gen, 7, 40, device=device), tensor(gen, 7, 40, device=device)
+    st = blocks.DropoutState(2, device=device)
+
+    def run(names):
+        t = {k: v.clone().requires_grad_(k in names) for k, v in base.items()}
+        out = blocks.residual_norm(t["x"], t["residual"], norm=blocks.Norm("layer", t["wo"], t["bo"]), norm_in=blocks.Norm("layer", t["wi"], t["bi"]), gate=t["gate"], p=0.2,
+                                   state=st.tensor, call=3, return_sum=True)
+        return dict(zip(names, torch.autograd.grad(out, [t[k] for k in names], [dy, ds])))
+    every = run(list(base))
+    for name in base:
+        assert torch.equal(run([name])[name], every[name]), name
+    # x = residual: s = 2 x; the gradients of both places add up
+    for p in (0.0, 0.3):
+        x, w = base["x"].clone().requires_grad_(), base["wo"].clone().requires_grad_()
+        y = blocks.residual_norm(x, x, norm=blocks.Norm("rms", w), norm_in=blocks.Norm("rms", w) if p else None, p=p, state=st.tensor, call=0)
+        gx, gw = torch.autograd.grad(y, [x, w], [dy])
+        ref = residual_norm_reference(x, x, ("rms", w, None, 1e-5), ("rms", w, None, 1e-5) if p else None, None, 1.0, p, (2, 0, 0), dy, None)
+        check(gx, ref["x"][0] + ref["residual"][0], ref["x"][1] + ref["residual"][1], what="dx of both places")
+        check(gw, ref["w_out"][0] + (ref["w_in"][0] if p else 0.0), ref["w_out"][1] + (ref["w_in"][1] if p else 0.0), what="dw of both places")
+    # table and weights apart; rows that the same entry names twice
+    tab, ix, wt = tensor(gen, 9, 16, device=device), torch.tensor([[1, 1, 4], [0, 4, 4]], device=device), torch.rand(2, 3, generator=gen).to(device)
+    g = tensor(gen, 2, 16, device=device)
+    both = [t.clone().requires_grad_() for t in (tab, wt)]
+    dt, dw = torch.autograd.grad(blocks.embedding(both[0], ix, weight=both[1]), both, [g])
+    t1, w1 = tab.clone().requires_grad_(), wt.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(blocks.embedding(t1, ix, weight=wt), [t1], [g])[0], dt)
+    assert torch.equal(torch.autograd.grad(blocks.embedding(tab, ix, weight=w1), [w1], [g])[0], dw)
+    ref = embedding_reference(tab, ix, wt, 1.0, None, g, True)
+    check(dt, *ref[1], what="dtable of repeated rows")
+
+
 def run_masked_rows(device):
     """everything dropped, rows of equal values, rows of the type's lowest value, infinities in dropped places"""
     from lidarseg3d_amd import blocks

@@ -40,6 +40,10 @@ def test_shapes_strides_and_absent_parts():
     bc.run_strides_and_absent_parts(DEV)
 
 
+def test_partial_gradients_and_shared_inputs():
+    bc.run_partial_gradients(DEV)
+
+
 def test_masked_rows_and_values():
     bc.run_masked_rows(DEV)
 

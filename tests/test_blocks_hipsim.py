@@ -66,6 +66,10 @@ def test_a_block_of_all_three_operators(device="cpu"):
     bc.run_block(device, rows=12, width=24, table=30)
 
 
+def test_partial_gradients_and_shared_inputs():
+    bc.run_partial_gradients("cpu")
+
+
 def test_masked_rows_and_values():
     bc.run_masked_rows("cpu")
 
