@@ -105,10 +105,10 @@ __global__ __launch_bounds__(256) void k_es_hist(emb_keys K, const uint2 *__rest
   if (FIRST) emb_clear<T>(dtable, elems, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
 
-// hist[workgroup][digit] -> the digit's count in the workgroups before, totals[digit]: 32 digits x 32 segments of workgroups per workgroup
+// hist[workgroup][digit] -> the digit's count in the workgroups before, totals[digit]: 16 digits x 64 segments of workgroups per workgroup
 __global__ __launch_bounds__(1024) void k_es_scan(int32_t *__restrict__ hist, int ntiles, int digits, int32_t *__restrict__ totals) {
-  __shared__ int s_seg[32][33];
-  const int d = blockIdx.x * 32 + (threadIdx.x & 31), seg = threadIdx.x >> 5, per = (ntiles + 31) / 32;
+  __shared__ int s_seg[64][17];
+  const int dig = threadIdx.x & 15, d = blockIdx.x * 16 + dig, seg = threadIdx.x >> 4, per = (ntiles + 63) / 64;
   const int lo = seg * per, hi = lo + per < ntiles ? lo + per : ntiles;
   const bool on = d < digits;
   int s = 0;
@@ -119,12 +119,12 @@ __global__ __launch_bounds__(1024) void k_es_scan(int32_t *__restrict__ hist, in
 #pragma unroll
     for (int q = 0; q < 16; ++q) s += v[q];
   }
-  s_seg[seg][threadIdx.x & 31] = s;
+  s_seg[seg][dig] = s;
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
-  for (int q = 0; q < 32; ++q) {
-    const int x = s_seg[q][threadIdx.x & 31];
+  for (int q = 0; q < 64; ++q) {
+    const int x = s_seg[q][dig];
     before += q < seg ? x : 0;
     total += x;
   }
@@ -557,7 +557,7 @@ static const uint2 *emb_sort(const emb_keys &K, int entries, const emb_space &S,
   do {                                                                                                                                                                  \
     hipLaunchKernelGGL((k_es_hist<T, FIRST_, ITEMS_>), dim3(GRID_), dim3(256), 0, stream, K, (const uint2 *)in, entries, (const int32_t *)n_valid, p * per, digits,      \
                        ntiles, hist, dtable, elems);                                                                                                                    \
-    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 31) / 32)), dim3(1024), 0, stream, hist, ntiles, digits, totals);                                            \
+    hipLaunchKernelGGL(k_es_scan, dim3((unsigned)((digits + 15) / 16)), dim3(1024), 0, stream, hist, ntiles, digits, totals);                                            \
     hipLaunchKernelGGL((k_es_scatter<FIRST_, ITEMS_>), dim3((unsigned)ntiles), dim3(256), 0, stream, K, (const uint2 *)in, entries, n_valid, p * per, digits, per,       \
                        (const int32_t *)hist, (const int32_t *)totals, out);                                                                                            \
   } while (0)
