@@ -3,7 +3,7 @@
     from lidarseg3d_amd import blocks
     rng = blocks.DropoutState(seed=0, device="cuda")
     h = blocks.embedding(table, tokens, scale=32.0)                                             # lookup, gradient by sorted tokens
-    h, y = blocks.residual_norm(block(y), h, norm=blocks.Norm.of(ln), p=0.1, state=rng, return_sum=True)  # h + dropout(block), its norm
+    y, h = blocks.residual_norm(block(y), h, norm=blocks.Norm.of(ln), p=0.1, state=rng, return_sum=True)  # the norm of h + dropout(block), and that sum
     y = blocks.dropout(linear(y), 0.1, rng, relu=True)                                          # dropout(relu(.))
     loss.backward(); rng.advance()
 
