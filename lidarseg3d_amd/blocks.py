@@ -19,6 +19,7 @@ from . import _lib, ops
 
 _KINDS = {"layer": 1, "rms": 2}
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_NO_NORM = (None, None, 0, 0.0)
 
 
 class Norm(object):
@@ -48,7 +49,8 @@ class Norm(object):
 class DropoutState(object):
     """(seed, step) of a training program's dropout, on the device, and the number of the next call within the step.  The kernels read seed and step
     when they run: a captured training step that ends with advance() draws new masks at every replay.  advance() comes after the backward pass
-    of everything drawn before it (an eager backward that finds another step raises, as after any in-place change of a saved tensor)."""
+    of everything drawn before it (an eager backward that finds another step raises, as after any in-place change of a saved tensor).  A graph keeps the call
+    numbers of its capture; eager work between its replays takes a state of its own, or it may draw what the graph draws."""
 
     def __init__(self, seed, device="cuda", step=0):
         self.tensor = torch.tensor([int(seed), int(step)], dtype=torch.int64, device=device)
@@ -83,11 +85,11 @@ def _on_device(t, what):
 
 def _draw(p, state, call):
     """-> (p, state tensor, call) of a dropout"""
+    if p == 0.0:
+        return 0.0, None, 0
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError("dropout probability %r" % (p,))
-    if p == 0.0:
-        return 0.0, None, 0
     if isinstance(state, DropoutState):
         call = state.next_call() if call is None else call
         state = state.tensor
@@ -106,8 +108,10 @@ def dropout(x, p, state, call=None, relu=False):
     again in the backward pass: it is never stored (relu: one bit per element says where x was positive and kept).
     p is resolved to 1 / 65536 and what is kept is scaled by the inverse of the resolved probability.  state: a DropoutState, or its tensor together with
     `call`; two dropouts of one step need different calls.  A dropped element is zero whatever stood there."""
-    _on_device(x, "dropout")
-    _dtype_ok(x, "dropout")
+    if not x.is_cuda:
+        _on_device(x, "dropout")
+    if x.dtype not in _TYPES:
+        _dtype_ok(x, "dropout")
     p, state, call = _draw(p, state, call)
     if p == 0.0:
         return torch.relu(x) if relu else x
@@ -115,7 +119,7 @@ def dropout(x, p, state, call=None, relu=False):
         return dropout(x.reshape(1), p, state, call, relu).reshape(())
     if x.numel() == 0:
         return x
-    return _lib.host_module().dropout(x, p, state, call, bool(relu))
+    return _lib.host_module().dropout(x, p, state, call, relu)
 
 
 class Dropout(nn.Dropout):
@@ -133,9 +137,7 @@ class Dropout(nn.Dropout):
 
 # ---------------------------------------------------------------------------------------------- residual, dropout, gate and norms
 def _norm_arguments(nm, c, what):
-    """-> weight, bias, kind, eps of a Norm or None, checked against rows of c values"""
-    if nm is None:
-        return None, None, 0, 0.0
+    """-> weight, bias, kind, eps of a Norm, checked against rows of c values"""
     if not isinstance(nm, Norm):
         raise TypeError("%s: a blocks.Norm needed, got %s" % (what, type(nm).__name__))
     out = []
@@ -158,17 +160,20 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
 
     norm / norm_in: a Norm (layer or RMS) or None.  gate: None, a single value, one per channel [c], or one per element (x's shape and type).
     residual: x's shape, of x's type or float32 (s has its type).  p / state / call: as in `dropout`; p = 0 outside training.  c <= 8192."""
-    _on_device(x, "residual_norm")
-    _dtype_ok(x, "residual_norm")
-    if x.dim() < 1:
+    if not x.is_cuda:
+        _on_device(x, "residual_norm")
+    if x.dtype not in _TYPES:
+        _dtype_ok(x, "residual_norm")
+    shape = x.shape
+    if not shape:
         raise ValueError("residual_norm needs at least one dimension")
-    shape, c = x.shape, x.shape[-1]
+    c = shape[-1]
     if c > 8192:
         raise ValueError("residual_norm takes rows of up to 8192 values, got %d" % c)
     if residual is not None:
         if residual.shape != shape:
             raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(shape)))
-        if residual.dtype not in (x.dtype, torch.float32):
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
             raise TypeError("residual: %s or float32 needed, got %s" % (x.dtype, residual.dtype))
     if gate is not None:
         _dtype_ok(gate, "gate")
@@ -181,11 +186,11 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
                 gate = gate.contiguous()
         else:
             raise ValueError("gate %s: one value, [%d] or %s" % (tuple(gate.shape), c, tuple(shape)))
-    w_in, b_in, kind_in, eps_in = _norm_arguments(norm_in, c, "norm_in")
-    w_out, b_out, kind_out, eps_out = _norm_arguments(norm, c, "norm")
+    w_in, b_in, kind_in, eps_in = _NO_NORM if norm_in is None else _norm_arguments(norm_in, c, "norm_in")
+    w_out, b_out, kind_out, eps_out = _NO_NORM if norm is None else _norm_arguments(norm, c, "norm")
     p, state, call = _draw(p, state, call)
-    out = _lib.host_module().residual_norm(x, residual, gate, w_in, b_in, w_out, b_out, state, kind_in, eps_in, kind_out, eps_out, float(alpha), p, call, bool(return_sum))
-    return tuple(out) if len(out) == 2 else out[0]
+    out = _lib.host_module().residual_norm(x, residual, gate, w_in, b_in, w_out, b_out, state, kind_in, eps_in, kind_out, eps_out, alpha, p, call, return_sum)
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 # ---------------------------------------------------------------------------------------------- row lookup
@@ -194,11 +199,13 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
     shape) the weighted sum, scale * sum_j weight[..., j] * table[idx[..., j]].  An index outside [0, rows) - -1 by custom - names no row: it reads as zero and takes no
     gradient.  padding_idx: a row that is read but takes no gradient.  The table's gradient is dense; its entries are sorted by row and
     added in input order: the same bits every time, for one frequent token as for many rare ones."""
-    _on_device(table, "embedding")
-    _dtype_ok(table, "embedding")
+    if not table.is_cuda:
+        _on_device(table, "embedding")
+    if table.dtype not in _TYPES:
+        _dtype_ok(table, "embedding")
     if table.dim() != 2:
         raise ValueError("embedding: a table [rows, c] needed, got %s" % (tuple(table.shape),))
-    if idx.dtype not in (torch.int32, torch.int64):
+    if idx.dtype != torch.int64 and idx.dtype != torch.int32:
         raise TypeError("embedding: int32 or int64 indices needed, got %s" % idx.dtype)
     if weight is not None:
         if weight.dtype != torch.float32:
@@ -212,11 +219,13 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
         raise ValueError("padding_idx %r outside a table of %d rows" % (padding_idx, table.shape[0]))
     padding = -1 if padding_idx is None else int(padding_idx) % table.shape[0]
     lead, k = (idx.shape[:-1], idx.shape[-1]) if bag else (idx.shape, 1)
-    if idx.dim() != 2 or not bag or not idx.is_contiguous():
+    if not bag and idx.dim() == 1 and idx.is_contiguous():
+        idx = idx.unsqueeze(1)
+    elif idx.dim() != 2 or not bag or not idx.is_contiguous():
         idx = idx.reshape(-1, k).contiguous()
     if weight is not None and (weight.dim() != 2 or not weight.is_contiguous()):
         weight = weight.reshape(-1, k).contiguous()
-    out = _lib.host_module().embedding(table, weight, idx, float(scale), padding)
+    out = _lib.host_module().embedding(table, weight, idx, scale, padding)
     return out if len(lead) == 1 else out.reshape(*lead, table.shape[1])
 
 

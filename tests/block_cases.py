@@ -370,6 +370,9 @@ def run_strides_and_absent_parts(device):
     t0 = torch.ones(4, 8, device=device, requires_grad=True)
     o0 = blocks.embedding(t0, torch.zeros(0, dtype=torch.int32, device=device))
     assert o0.shape == (0, 8) and bool((torch.autograd.grad(o0, [t0], [torch.zeros(0, 8, device=device)])[0] == 0).all())
+    tz = torch.ones(0, 8, device=device, requires_grad=True)
+    oz = blocks.embedding(tz, torch.tensor([0, 3, -1], device=device))
+    assert oz.shape == (3, 8) and bool((oz == 0).all()) and torch.autograd.grad(oz.sum(), [tz])[0].shape == (0, 8)
     on = blocks.embedding(t0, torch.full((5,), -1, device=device))
     assert bool((on == 0).all()) and bool((torch.autograd.grad(on.sum(), [t0])[0] == 0).all())
 
