@@ -18,8 +18,8 @@ __device__ __forceinline__ long long emb_index(const void *__restrict__ idx, int
 }
 
 // One chunk of 8 columns of one output row per thread; I: 32 bits where the chunk count allows.  A lookup is a chain of two round trips (index, table row), so
-// U entries of a row that sums several are kept in flight.  (k = 1: four rows a thread in flight on 2048 workgroups or one on up to 16384 make no difference,
-// 360000 x 64 f32 26.5 / 24.8 us.)
+// U entries of a row that sums several are kept in flight.  Up to 16384 workgroups, few trips a thread: with 2048, 360000 x 64 f32, k = 1 took 26.5 us instead of
+// 24.8, and 360000 x 48 f32, k = 8 took 7 us longer (eight entries in flight are no faster than four).
 template <typename T, typename I, int U>
 __global__ __launch_bounds__(256) void k_emb_fwd(const T *__restrict__ table, size_t table_ld, long long rows, int c, const void *__restrict__ idx, int is64, I total, int k,
                                                  const float *__restrict__ weight, float scale, T *__restrict__ out) {
@@ -486,12 +486,11 @@ extern "C" int ls3d_embedding_forward(const void *table, long long table_ld, lon
   const long long total = (long long)n * ((c + 7) / 8);
   const int is64 = idx_dtype == LS3D_INDEX_I64;
 #define EMB_FWD(I_, U_)                                                                                                                                                   \
-  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, I_, U_>), ls3d_grid(total, 256, U_ == 1 ? 16384 : 2048), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (I_)total, k, \
+  EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_fwd<T, I_, U_>), ls3d_grid(total, 256, 16384), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64, (I_)total, k, \
                                       weight, scale, (T *)out))
   if (total < (1ll << 30)) {  // (the strides on top stay below 2^32)
     if (k == 1) EMB_FWD(uint32_t, 1);
-    else if (k <= 4) EMB_FWD(uint32_t, 4);
-    else EMB_FWD(uint32_t, 8);
+    else EMB_FWD(uint32_t, 4);
   } else EMB_FWD(unsigned long long, 4);
 #undef EMB_FWD
   LS3D_RETURN_IF_LAUNCH_FAILED();
