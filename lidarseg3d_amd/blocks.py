@@ -50,13 +50,16 @@ class DropoutState(object):
     """(seed, step) of a training program's dropout, on the device, and the number of the next call within the step.  The kernels read seed and step
     when they run: a captured training step that ends with advance() draws new masks at every replay.  advance() comes after the backward pass
     of everything drawn before it (an eager backward that finds another step raises, as after any in-place change of a saved tensor).  A graph keeps the call
-    numbers of its capture; eager work between its replays takes a state of its own, or it may draw what the graph draws."""
+    numbers of its capture; eager work between its replays takes a state of its own, or it may draw what the graph draws.  Under activation checkpointing
+    each dropout is given its `call`: a forward pass repeated inside the backward pass that asks for the next number raises."""
 
     def __init__(self, seed, device="cuda", step=0):
         self.tensor = torch.tensor([int(seed), int(step)], dtype=torch.int64, device=device)
         self.calls = 0
 
     def next_call(self):
+        if torch._C._current_graph_task_id() != -1:  # (activation checkpointing: the forward pass is repeated and would count on, its masks not those of the first time)
+            raise RuntimeError("a dropout inside a backward pass (activation checkpointing) needs its `call` given")
         n = self.calls
         self.calls += 1
         return n

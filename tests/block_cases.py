@@ -591,3 +591,33 @@ def run_use_in_training(device):
     assert state.calls == 1 and 0 < int((y == 0).sum()) < y.numel() and torch.equal(drops[0].eval()(x), x)
     blocks.use_in_training(model, None)
     assert model.point_head.block_state is None and all(m.state is None for m in drops)
+
+
+def run_checkpointing(device, reentrant):
+    import pytest
+    from torch.utils.checkpoint import checkpoint
+
+    from lidarseg3d_amd import blocks
+    torch.manual_seed(5)
+    x, r, w = (torch.randn(s).to(device).requires_grad_() for s in ((37, 24), (37, 24), (24,)))
+    dy = torch.randn(37, 24).to(device)
+    state = blocks.DropoutState(11, device=device)
+
+    def block(x, r, calls=(None, None)):
+        h = blocks.dropout(x, 0.3, state, call=calls[0], relu=True)
+        return blocks.residual_norm(h, r, norm=blocks.Norm("rms", w, None, 1e-5), p=0.2, state=state, call=calls[1])
+
+    y = block(x, r)
+    want = torch.autograd.grad(y, (x, r, w), dy)
+    state.calls = 0
+    for t in (x, r, w):
+        t.grad = None
+    z = checkpoint(block, x, r, (0, 1), use_reentrant=reentrant)
+    z.backward(dy)
+    assert torch.equal(y, z) and all(torch.equal(t.grad, g) for t, g in zip((x, r, w), want))
+    z = checkpoint(block, x, r, use_reentrant=reentrant)
+    assert torch.equal(y, z)
+    with pytest.raises(RuntimeError, match="activation checkpointing"):
+        z.backward(dy)
+    assert state.calls == 2
+    torch.autograd.grad(block(x, r), (x, r, w), dy)  # the engine is none the worse

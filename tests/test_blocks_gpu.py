@@ -220,3 +220,8 @@ def test_large_passes_equal_their_parts():
         assert torch.equal(z[:64], want)
         assert torch.equal(z[:9000], blocks.dropout(big[:9000], 0.3, st.tensor, call=5, relu=True))
         del big, z
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activation_checkpointing(reentrant):
+    bc.run_checkpointing(DEV, reentrant)

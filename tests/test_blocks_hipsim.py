@@ -218,3 +218,9 @@ def test_argument_errors_of_the_c_entry_points():
     assert eb() == 0
     for bad, code in ((dict(do=None), ARG), (dict(old=7), ARG), (dict(ws=None), ARG), (dict(wsb=64), WS), (dict(ws=P(big, 4)), ARG), (dict(dw=P(dw)), ARG)):
         assert eb(**bad) == code, bad
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activation_checkpointing(reentrant):
+    """a repeated forward pass draws the masks of the first with `call` given, and is refused where it would count on"""
+    bc.run_checkpointing("cpu", reentrant)
