@@ -67,7 +67,6 @@ Tensor rows(const Tensor &t) {
 long long ld(const Tensor &t) { return t.defined() ? (t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1)) : 0; }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor fresh(const Tensor &like, at::IntArrayRef sizes) { return at::empty(sizes, like.options()); }
-Tensor shaped(const Tensor &t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
 Tensor tensor(const Optional &t) { return t.has_value() ? *t : Tensor(); }
 Optional maybe(const Tensor &t) { return t.defined() ? Optional(t) : c10::nullopt; }  // (a Function's absent inputs: they have no place among its edges)
 void *stream(const Tensor &t) { return t.is_cuda() ? (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream() : nullptr; }  // (the host emulation: none)
@@ -151,15 +150,15 @@ ls3d_residual_norm_t descriptor(const NormForm &f, const Tensor &x, const Tensor
   return d;
 }
 
-// x, residual, gate: rows [n, c] (gate also [c]) -> y, s, stats (undefined where not wanted)
-std::array<Tensor, 3> norm_raw(const NormForm &f, const Tensor &x, const Tensor &residual, const Tensor &gate, const Tensor &w_in, const Tensor &b_in, const Tensor &w_out,
+// x, residual, gate: rows [n, c] (gate also [c]) -> y, s of the caller's shape, stats (undefined where not wanted)
+std::array<Tensor, 3> norm_raw(const NormForm &f, at::IntArrayRef shape, const Tensor &x, const Tensor &residual, const Tensor &gate, const Tensor &w_in, const Tensor &b_in, const Tensor &w_out,
                                const Tensor &b_out, const Tensor &state, bool want_stats) {
   same_device(x, {&residual, &gate, &w_in, &b_in, &w_out, &b_out, &state});
   const c10::DeviceGuard guard(x.device());
   const ls3d_residual_norm_t d = descriptor(f, x, residual, gate, w_in, b_in, w_out, b_out, state);
   Tensor y, s, stats;
-  if (f.kind_out) y = fresh(x, x.sizes());
-  if (f.want_sum || !f.kind_out) s = fresh(residual.defined() ? residual : x, x.sizes());
+  if (f.kind_out) y = fresh(x, shape);
+  if (f.want_sum || !f.kind_out) s = fresh(residual.defined() ? residual : x, shape);
   if (want_stats) stats = at::empty({x.size(0), 4}, x.options().dtype(at::kFloat));
   check(api.norm_forward(ptr(x), ld(x), ptr(residual), ld(residual), count(x.size(0)), count(x.size(1)), &d, ptr(y), ptr(s), stats.defined() ? stats.data_ptr<float>() : nullptr,
                          stream(x)), "ls3d_residual_norm_forward");
@@ -170,13 +169,18 @@ variable_list norm_outputs(const NormForm &f, const std::array<Tensor, 3> &o) {
   return {f.kind_out ? o[0] : o[1]};
 }
 
+Tensor gate_rows(const Tensor &g) { return g.defined() ? g.dim() == 1 ? g.contiguous() : rows(g) : Tensor(); }
+
+// Takes the caller's tensors and makes rows of them inside: a gradient goes back as the one tensor that the kernel wrote.  Views of it, as a reshape before the
+// Function would make, look like tensors of their own to the engine, which then keeps and adds to each as if no other shared its memory.
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list forward(AutogradContext *ctx, const Tensor &x, const Optional &residual, const Optional &gate, const Optional &w_in, const Optional &b_in,
                                const Optional &w_out, const Optional &b_out, const Optional &state, const NormForm &f) {
-    const Tensor t[] = {x, tensor(residual), tensor(gate), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out), tensor(state)};
-    const auto o = norm_raw(f, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], true);
+    const Tensor t[] = {rows(x), residual ? rows(*residual) : Tensor(), gate_rows(tensor(gate)), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out), tensor(state)};
+    const auto o = norm_raw(f, x.sizes(), t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], true);
     ctx->save_for_backward({t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], o[2]});
     ctx->saved_data["f"] = f.pack();
+    ctx->saved_data["shape"] = x.sizes().vec();
     ctx->set_materialize_grads(false);
     return norm_outputs(f, o);
   }
@@ -191,6 +195,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     variable_list out(9);
     if (!dy.defined() && !ds.defined()) return out;
     const auto v = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
     const Tensor &x = v[0], &residual = v[1], &gate = v[2];
     const c10::DeviceGuard guard(x.device());
     if (dy.defined()) dy = rows(dy);
@@ -201,7 +206,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const bool same = want[0] && want[1] && !gate.defined() && !f.kind_in && f.p == 0.0 && f.alpha == 1.0 && x.scalar_type() == residual.scalar_type();
     if (same) want[0] = false;
     for (int i = 0; i < 7; ++i)
-      if (want[i]) out[i] = fresh(v[i], v[i].sizes());
+      if (want[i]) out[i] = fresh(v[i], i < 2 || (i == 2 && gate.dim() > 1) ? at::IntArrayRef(shape) : v[i].sizes());
     const int n = count(x.size(0)), c = count(x.size(1));
     const size_t bytes = api.norm_workspace(n, c);
     Tensor ws;
@@ -217,14 +222,11 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 variable_list residual_norm(const Tensor &x, const Optional &residual, const Optional &gate, const Optional &w_in, const Optional &b_in, const Optional &w_out, const Optional &b_out,
                             const Optional &state, int64_t kind_in, double eps_in, int64_t kind_out, double eps_out, double alpha, double p, int64_t call, bool want_sum) {
   const NormForm f = {kind_in, kind_out, call, eps_in, eps_out, alpha, p, want_sum};
-  const Tensor x2 = rows(x), r2 = residual ? rows(*residual) : Tensor(), g2 = gate ? (gate->dim() == 1 ? gate->contiguous() : rows(*gate)) : Tensor();
-  const Tensor t[] = {x2, r2, g2, tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out)};
+  const Tensor t[] = {x, tensor(residual), tensor(gate), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out)};
   bool grad = false;
   for (const Tensor &u : t) grad = grad || (u.defined() && u.requires_grad());
-  variable_list out = grad && at::GradMode::is_enabled() ? ResidualNorm::apply(t[0], maybe(t[1]), maybe(t[2]), maybe(t[3]), maybe(t[4]), maybe(t[5]), maybe(t[6]), state, f)
-                                                          : norm_outputs(f, norm_raw(f, t[0], t[1], t[2], t[3], t[4], t[5], t[6], tensor(state), false));
-  for (Tensor &o : out) o = shaped(o, x.sizes());
-  return out;
+  if (grad && at::GradMode::is_enabled()) return ResidualNorm::apply(x, maybe(t[1]), maybe(t[2]), maybe(t[3]), maybe(t[4]), maybe(t[5]), maybe(t[6]), state, f);
+  return norm_outputs(f, norm_raw(f, x.sizes(), rows(x), t[1].defined() ? rows(t[1]) : Tensor(), gate_rows(t[2]), t[3], t[4], t[5], t[6], tensor(state), false));
 }
 
 // ---------------------------------------------------------------------------------------------- row lookup

@@ -621,3 +621,29 @@ def run_checkpointing(device, reentrant):
         z.backward(dy)
     assert state.calls == 2
     torch.autograd.grad(block(x, r), (x, r, w), dy)  # the engine is none the worse
+
+
+def run_accumulated_gradients(device):
+    """.grad of leaves of one, two and three dimensions over two backward passes: twice the single gradient, in memory of its own for each leaf, whatever x and the
+    residual share inside (a plain sum has one gradient for both)"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(31)
+    for shape in ((24,), (5, 24), (2, 3, 24)):
+        for norm in (None, blocks.Norm("layer")):
+            x, r = (tensor(gen, *shape, device=device).requires_grad_() for _ in range(2))
+            dy = tensor(gen, *shape, device=device)
+            f = lambda: blocks.residual_norm(x, r, norm=norm)
+            once = torch.autograd.grad(f(), [x, r], [dy])
+            for _ in range(2):
+                f().backward(dy)
+            assert x.grad.data_ptr() != r.grad.data_ptr(), shape
+            for t, g in zip((x, r), once):
+                assert t.grad.shape == t.shape and torch.equal(t.grad, 2 * g), shape
+        # both leaves through other operators, and a leaf that is x and residual at once
+        x, r = (tensor(gen, *shape, device=device).requires_grad_() for _ in range(2))
+        blocks.residual_norm(2 * x, 4 * r).backward(dy)
+        assert torch.equal(x.grad, 2 * dy) and torch.equal(r.grad, 4 * dy)
+        x.grad = None
+        for _ in range(2):
+            blocks.residual_norm(x, x).backward(dy)
+        assert torch.equal(x.grad, 4 * dy)

@@ -225,3 +225,7 @@ def test_large_passes_equal_their_parts():
 @pytest.mark.parametrize("reentrant", [False, True])
 def test_activation_checkpointing(reentrant):
     bc.run_checkpointing(DEV, reentrant)
+
+
+def test_accumulated_gradients():
+    bc.run_accumulated_gradients(DEV)

@@ -224,3 +224,7 @@ def test_argument_errors_of_the_c_entry_points():
 def test_activation_checkpointing(reentrant):
     """a repeated forward pass draws the masks of the first with `call` given, and is refused where it would count on"""
     bc.run_checkpointing("cpu", reentrant)
+
+
+def test_accumulated_gradients():
+    bc.run_accumulated_gradients("cpu")
