@@ -610,7 +610,8 @@ extern "C" int ls3d_embedding_backward(const void *table, long long table_ld, lo
     if (!workspace || ((uintptr_t)workspace & 15)) return LS3D_ERR_ARG;
     if (workspace_bytes < ls3d_embedding_workspace_bytes(n, k, c)) return LS3D_ERR_WORKSPACE;
   }
-  if (dweight && entries > 0 && c > 0) {
+  if (dweight && entries > 0 && (!idx || ((uintptr_t)idx & (is64 ? 7 : 3)))) return LS3D_ERR_ARG;
+  if (dweight && entries > 0) {  // (c = 0: the products of no columns, zeros; no row is read)
     int lpr = 1;
     while (lpr * 8 < c && lpr < 64) lpr *= 2;
     EMB_TYPES(dtype, hipLaunchKernelGGL((k_emb_dweight<T>), ls3d_grid(entries, 256 / lpr), dim3(256), 0, stream, (const T *)table, (size_t)table_ld, rows, c, idx, is64,

@@ -647,3 +647,17 @@ def run_accumulated_gradients(device):
         for _ in range(2):
             blocks.residual_norm(x, x).backward(dy)
         assert torch.equal(x.grad, 4 * dy)
+
+
+def run_weight_gradient_of_no_columns(device):
+    """a table without columns: the weights' gradient is a product over nothing, zeros in memory that held something else before"""
+    from lidarseg3d_amd import blocks
+    for T in (F32, BF16):
+        for ix in (torch.tensor([[1, 1], [0, 4], [-1, 9]]), torch.zeros(2, 3, 700, dtype=torch.int64)):
+            junk = [torch.full(ix.shape, 7.0, device=device) for _ in range(4)]
+            del junk
+            table, w = torch.zeros(5, 0, dtype=T, device=device, requires_grad=True), torch.rand(ix.shape).to(device).requires_grad_()
+            y = blocks.embedding(table, ix.to(device), weight=w)
+            assert y.shape == (*ix.shape[:-1], 0)
+            dt, dw = torch.autograd.grad(y.sum(), [table, w])
+            assert dt.shape == (5, 0) and torch.equal(dw, torch.zeros_like(w))

@@ -229,3 +229,7 @@ def test_activation_checkpointing(reentrant):
 
 def test_accumulated_gradients():
     bc.run_accumulated_gradients(DEV)
+
+
+def test_weight_gradient_of_no_columns():
+    bc.run_weight_gradient_of_no_columns(DEV)

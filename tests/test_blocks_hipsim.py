@@ -228,3 +228,17 @@ def test_activation_checkpointing(reentrant):
 
 def test_accumulated_gradients():
     bc.run_accumulated_gradients("cpu")
+
+
+def test_weight_gradient_of_no_columns():
+    bc.run_weight_gradient_of_no_columns("cpu")
+
+
+def test_c_entry_of_a_weight_gradient_of_no_columns():
+    """the indices are checked there too: they are read"""
+    import ctypes
+    L, ll, dw, idx = _lib.load(), ctypes.c_longlong, torch.full((8,), 7.0), torch.zeros(9, dtype=torch.int64)
+    call = lambda ix: L.ls3d_embedding_backward(None, ll(0), ll(5), 0, 0, ix, 1, 8, 1, None, ctypes.c_float(1.0), ll(-1), None, ll(0), None, ctypes.c_void_p(dw.data_ptr()),
+                                                None, ctypes.c_size_t(0), None)
+    assert call(None) == -1 and call(ctypes.c_void_p(idx.data_ptr() + 4)) == -1 and bool((dw == 7).all())
+    assert call(ctypes.c_void_p(idx.data_ptr())) == 0 and bool((dw == 0).all())
