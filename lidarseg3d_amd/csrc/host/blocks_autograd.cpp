@@ -78,6 +78,12 @@ void same_device(const Tensor &ref, std::initializer_list<const Tensor *> others
   for (const Tensor *t : others) TORCH_CHECK(!t->defined() || t->device() == ref.device(), "tensors on different devices: ", ref.device(), " and ", t->device());
 }
 
+// What would be lost without a word: tangents of forward-mode differentiation (the inputs of a call, the gradients that come into a backward pass)
+void usable(const char *what, at::ArrayRef<Tensor> tensors) {
+  for (const Tensor &t : tensors)
+    if (t.defined()) TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative (an input carries a tangent)");
+}
+
 // ---------------------------------------------------------------------------------------------- dropout
 Tensor dropout_raw(const Tensor &x, double p, const Tensor &state, int64_t call, bool relu, Tensor *bits) {
   same_device(x, {&state});
@@ -100,6 +106,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once("dropout");
+    usable("dropout", grads);
     const auto saved = ctx->get_saved_variables();
     const auto a = ctx->saved_data["a"].toDoubleVector();
     const c10::DeviceGuard guard(grads[0].device());
@@ -112,6 +119,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor &x, double p, const Tensor &state, int64_t call, bool relu) {
+  usable("dropout", x);
   if (at::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, p, state, call, relu);
   return dropout_raw(x, p, state, call, relu, nullptr);
 }
@@ -186,6 +194,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once("residual_norm");
+    usable("residual_norm", grads);
     const NormForm f = NormForm::unpack(ctx->saved_data["f"].toDoubleVector());
     Tensor dy, ds;
     if (f.kind_out) {
@@ -223,6 +232,7 @@ variable_list residual_norm(const Tensor &x, const Optional &residual, const Opt
                             const Optional &state, int64_t kind_in, double eps_in, int64_t kind_out, double eps_out, double alpha, double p, int64_t call, bool want_sum) {
   const NormForm f = {kind_in, kind_out, call, eps_in, eps_out, alpha, p, want_sum};
   const Tensor t[] = {x, tensor(residual), tensor(gate), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out)};
+  usable("residual_norm", t);
   bool grad = false;
   for (const Tensor &u : t) grad = grad || (u.defined() && u.requires_grad());
   if (grad && at::GradMode::is_enabled()) return ResidualNorm::apply(x, maybe(t[1]), maybe(t[2]), maybe(t[3]), maybe(t[4]), maybe(t[5]), maybe(t[6]), state, f);
@@ -247,6 +257,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     once("embedding");
+    usable("embedding", grads);
     const auto v = ctx->get_saved_variables();
     const auto a = ctx->saved_data["a"].toDoubleVector();
     const Tensor &table = v[0], &weight = v[1], &idx = v[2];
@@ -270,6 +281,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 
 // idx [n, k], weight [n, k] or none -> [n, c]
 Tensor embedding(const Tensor &table, const Optional &weight, const Tensor &idx, double scale, int64_t padding) {
+  usable("embedding", {table, tensor(weight)});
   const Tensor t = rows(table), w = tensor(weight);
   if (at::GradMode::is_enabled() && (t.requires_grad() || (w.defined() && w.requires_grad()))) return Embedding::apply(t, maybe(w), idx, scale, padding);
   return embedding_raw(t, w, idx, scale);

@@ -661,3 +661,34 @@ def run_weight_gradient_of_no_columns(device):
             assert y.shape == (*ix.shape[:-1], 0)
             dt, dw = torch.autograd.grad(y.sum(), [table, w])
             assert dt.shape == (5, 0) and torch.equal(dw, torch.zeros_like(w))
+
+
+def operator_calls(device):
+    """name -> a call of one input [4, 8] of each operator"""
+    from lidarseg3d_amd import blocks
+    st = blocks.DropoutState(1, device=device)
+    ix, wt = torch.tensor([0, 3, 3], device=device), torch.ones(3, 2, device=device)
+    return {"dropout": lambda x: blocks.dropout(x, 0.5, st.tensor, call=0), "relu dropout": lambda x: blocks.dropout(x, 0.5, st.tensor, call=0, relu=True),
+            "residual_norm": lambda x: blocks.residual_norm(torch.ones_like(x), x, norm=blocks.Norm("layer"), p=0.5, state=st.tensor, call=1),
+            "norm weight": lambda x: blocks.residual_norm(torch.ones(3, 8, device=device), norm=blocks.Norm("rms", x.sum(0))),
+            "gate": lambda x: blocks.residual_norm(torch.ones(4, 8, device=device), gate=x),
+            "embedding": lambda x: blocks.embedding(x, ix), "lookup weights": lambda x: blocks.embedding(torch.ones(5, 6, device=device), torch.zeros(4, 8, dtype=torch.int64, device=device), weight=x)}
+
+
+def run_forward_mode(device):
+    """a tangent is refused wherever it comes in - inputs, parameters, the gradients of a backward pass - and the calls work again afterwards"""
+    import pytest
+    import torch.autograd.forward_ad as fw
+    for name, f in operator_calls(device).items():
+        for wants_grad in (False, True):
+            with fw.dual_level():
+                x = torch.randn(4, 8).to(device).requires_grad_(wants_grad)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(fw.make_dual(x, torch.ones_like(x)))
+        x = torch.randn(4, 8).to(device).requires_grad_()
+        y = f(x)
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, [x], [fw.make_dual(torch.ones_like(y), torch.ones_like(y))], retain_graph=True)
+            assert torch.isfinite(f(x)).all()  # no tangent: an ordinary call
+        assert torch.isfinite(torch.autograd.grad(y, [x], [torch.ones_like(y)])[0]).all()

@@ -233,3 +233,7 @@ def test_accumulated_gradients():
 
 def test_weight_gradient_of_no_columns():
     bc.run_weight_gradient_of_no_columns(DEV)
+
+
+def test_forward_mode_is_refused():
+    bc.run_forward_mode(DEV)

@@ -242,3 +242,7 @@ def test_c_entry_of_a_weight_gradient_of_no_columns():
                                                 None, ctypes.c_size_t(0), None)
     assert call(None) == -1 and call(ctypes.c_void_p(idx.data_ptr() + 4)) == -1 and bool((dw == 7).all())
     assert call(ctypes.c_void_p(idx.data_ptr())) == 0 and bool((dw == 0).all())
+
+
+def test_forward_mode_is_refused():
+    bc.run_forward_mode("cpu")
