@@ -8,7 +8,10 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../../include/ls3d.h"
 
@@ -78,10 +81,25 @@ void same_device(const Tensor &ref, std::initializer_list<const Tensor *> others
   for (const Tensor *t : others) TORCH_CHECK(!t->defined() || t->device() == ref.device(), "tensors on different devices: ", ref.device(), " and ", t->device());
 }
 
-// What would be lost without a word: tangents of forward-mode differentiation (the inputs of a call, the gradients that come into a backward pass)
+// A tracer sees the allocation of an output and not the kernel that fills it: what it records returns memory that nobody wrote
+bool traced() {
+  if (torch::jit::tracer::isTracing()) return true;
+  typedef c10::impl::TorchDispatchModeTLS Modes;
+  typedef c10::impl::TorchDispatchModeKey Key;
+  return Modes::any_modes_set() && (Modes::get_mode(Key::PROXY).has_value() || Modes::get_mode(Key::FAKE).has_value() || Modes::get_mode(Key::FUNCTIONAL).has_value());
+}
+// fake tensors, the wrappers of vmap, grad and functionalization
+bool in_memory(const Tensor &t) { return t.numel() == 0 || (t.has_storage() && t.storage().unsafeGetStorageImpl()->_mutable_data_ptr_no_checks().get()); }
+
+// What would give wrong answers or be lost without a word, of a call's inputs and of the gradients that come into a backward pass: a tracer that records,
+// tensors without memory of their own, tangents of forward-mode differentiation
 void usable(const char *what, at::ArrayRef<Tensor> tensors) {
-  for (const Tensor &t : tensors)
-    if (t.defined()) TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative (an input carries a tangent)");
+  TORCH_CHECK(!traced(), what, " cannot be traced (torch.jit.trace, make_fx, torch.export, fake tensors): a tracer does not see its kernels");
+  for (const Tensor &t : tensors) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(in_memory(t), what, " needs tensors in memory: fake tensors and the wrappers of torch.func (vmap, grad, jvp, functionalize) and batched gradients have none");
+    TORCH_CHECK(!t._fw_grad(0).defined(), what, " has no forward-mode derivative (an input carries a tangent)");
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- dropout
@@ -119,7 +137,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor &x, double p, const Tensor &state, int64_t call, bool relu) {
-  usable("dropout", x);
+  usable("dropout", {x, state});
   if (at::GradMode::is_enabled() && x.requires_grad()) return Dropout::apply(x, p, state, call, relu);
   return dropout_raw(x, p, state, call, relu, nullptr);
 }
@@ -233,6 +251,7 @@ variable_list residual_norm(const Tensor &x, const Optional &residual, const Opt
   const NormForm f = {kind_in, kind_out, call, eps_in, eps_out, alpha, p, want_sum};
   const Tensor t[] = {x, tensor(residual), tensor(gate), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out)};
   usable("residual_norm", t);
+  usable("residual_norm", tensor(state));
   bool grad = false;
   for (const Tensor &u : t) grad = grad || (u.defined() && u.requires_grad());
   if (grad && at::GradMode::is_enabled()) return ResidualNorm::apply(x, maybe(t[1]), maybe(t[2]), maybe(t[3]), maybe(t[4]), maybe(t[5]), maybe(t[6]), state, f);
@@ -281,7 +300,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 
 // idx [n, k], weight [n, k] or none -> [n, c]
 Tensor embedding(const Tensor &table, const Optional &weight, const Tensor &idx, double scale, int64_t padding) {
-  usable("embedding", {table, tensor(weight)});
+  usable("embedding", {table, tensor(weight), idx});
   const Tensor t = rows(table), w = tensor(weight);
   if (at::GradMode::is_enabled() && (t.requires_grad() || (w.defined() && w.requires_grad()))) return Embedding::apply(t, maybe(w), idx, scale, padding);
   return embedding_raw(t, w, idx, scale);

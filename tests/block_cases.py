@@ -692,3 +692,46 @@ def run_forward_mode(device):
                 torch.autograd.grad(y, [x], [fw.make_dual(torch.ones_like(y), torch.ones_like(y))], retain_graph=True)
             assert torch.isfinite(f(x)).all()  # no tangent: an ordinary call
         assert torch.isfinite(torch.autograd.grad(y, [x], [torch.ones_like(y)])[0]).all()
+
+
+def run_tracers_and_wrapped_tensors(device):
+    """torch.jit.trace, make_fx and fake tensors, torch.func's transforms, batched gradients: refused with the reason; ordinary calls work again afterwards, also under a
+    dispatch mode that only looks on"""
+    import warnings
+
+    import pytest
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Onlooker(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for name, f in operator_calls(device).items():
+        x = torch.randn(4, 8).to(device)
+        want = f(x)
+        for wants_grad in (False, True):
+            leaf = x.clone().requires_grad_(wants_grad)
+            with warnings.catch_warnings():
+                warnings.simplefilter("ignore")
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    torch.jit.trace(f, leaf, check_trace=False)
+            for mode in ("real", "fake"):
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    make_fx(f, tracing_mode=mode, _allow_non_fake_inputs=True)(leaf)
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            fake = mode.from_tensor(x)
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                f(fake)
+        for call in (lambda: f(fake), lambda: torch.func.vmap(f)(torch.stack([x, x])), lambda: torch.func.grad(lambda t: f(t).sum())(x),
+                     lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.functionalize(f)(x)):
+            with pytest.raises(RuntimeError, match="needs tensors in memory"):
+                call()
+        leaf = x.clone().requires_grad_()
+        y = f(leaf)
+        with pytest.raises(RuntimeError, match="needs tensors in memory"):
+            torch.autograd.grad(y, [leaf], [torch.ones(2, *y.shape, device=device)], is_grads_batched=True, retain_graph=True)
+        with Onlooker():
+            assert torch.equal(f(x), want)
+        assert torch.equal(f(x), want) and torch.isfinite(torch.autograd.grad(y, [leaf], [torch.ones_like(y)])[0]).all()

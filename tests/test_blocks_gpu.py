@@ -237,3 +237,7 @@ def test_weight_gradient_of_no_columns():
 
 def test_forward_mode_is_refused():
     bc.run_forward_mode(DEV)
+
+
+def test_tracers_and_wrapped_tensors_are_refused():
+    bc.run_tracers_and_wrapped_tensors(DEV)

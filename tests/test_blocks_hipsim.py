@@ -246,3 +246,7 @@ def test_c_entry_of_a_weight_gradient_of_no_columns():
 
 def test_forward_mode_is_refused():
     bc.run_forward_mode("cpu")
+
+
+def test_tracers_and_wrapped_tensors_are_refused():
+    bc.run_tracers_and_wrapped_tensors("cpu")
