@@ -127,6 +127,7 @@ def dropout(x, p, state, call=None, relu=False):
 
 class Dropout(nn.Dropout):
     """nn.Dropout on `dropout` with a DropoutState (None: torch's generator, as nn.Dropout); evaluation passes its input through"""
+    converted = False  # an nn.Dropout that use_in_training put on the operator
 
     def __init__(self, p, state=None):
         super().__init__(p)
@@ -135,7 +136,10 @@ class Dropout(nn.Dropout):
     def forward(self, input):
         if self.state is None:
             return super().forward(input)
-        return dropout(input, self.p, self.state) if self.training else input
+        if not self.training:
+            return input
+        out = dropout(input, self.p, self.state)
+        return input.copy_(out) if self.inplace and out is not input else out
 
 
 # ---------------------------------------------------------------------------------------------- residual, dropout, gate and norms
@@ -241,13 +245,13 @@ def use_in_training(model, state):
     calls state.advance() after each backward pass.  state None: back to the torch composition.  -> model"""
     if state is not None and not isinstance(state, DropoutState):
         raise TypeError("use_in_training: a DropoutState or None needed, got %s" % type(state).__name__)
-    for module in list(model.modules()):
+    for module in model.modules():
         if hasattr(type(module), "block_state"):
             module.block_state = state
+        if type(module) is nn.Dropout and state is not None:  # the same object: its hooks and every other place that holds it stay with it
+            module.__class__, module.converted = Dropout, True
         if isinstance(module, Dropout):
             module.state = state
-        for name, child in list(module.named_children()):
-            if type(child) is nn.Dropout and state is not None:
-                child = Dropout(child.p, state).train(child.training)
-                setattr(module, name, child)
+            if state is None and module.converted:
+                module.__class__, module.converted = nn.Dropout, False
     return model

@@ -735,3 +735,51 @@ def run_tracers_and_wrapped_tensors(device):
         with Onlooker():
             assert torch.equal(f(x), want)
         assert torch.equal(f(x), want) and torch.isfinite(torch.autograd.grad(y, [leaf], [torch.ones_like(y)])[0]).all()
+
+
+def run_converted_dropouts(device):
+    """use_in_training keeps a dropout's identity: hooks, names that share one module, a bare nn.Dropout as the model, in-place work; None gives back nn.Dropout"""
+    import copy
+
+    from lidarseg3d_amd import blocks
+    nn = torch.nn
+
+    class Twice(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = self.b = nn.Dropout(0.5)
+            self.seq = nn.Sequential(nn.Identity(), self.a, nn.Dropout(0.25, inplace=True), nn.Dropout(0.25).eval())
+            self.own = blocks.Dropout(0.5)
+
+    class Special(nn.Dropout):
+        pass
+    m, seen = Twice(), []
+    m.special = Special(0.5)
+    before = dict(m.named_modules(remove_duplicate=False))
+    m.a.register_forward_hook(lambda mod, i, o: seen.append("hook"))
+    state, x = blocks.DropoutState(3, device=device), torch.ones(64, 32, device=device)
+    blocks.use_in_training(m, state)
+    assert all(mod is before[name] for name, mod in m.named_modules(remove_duplicate=False)) and m.a is m.b is m.seq[1] and isinstance(m.a, nn.Dropout)
+    assert type(m.special) is Special and not m.seq[3].training and torch.equal(m.seq[3](x), x)
+    y, z = m.a(x), m.b(x)
+    assert state.calls == 2 and seen == ["hook", "hook"] and not torch.equal(y, z)
+    assert torch.equal(y, blocks.dropout(x, 0.5, state.tensor, call=0)) and torch.equal(z, blocks.dropout(x, 0.5, state.tensor, call=1))
+    t = x.clone()
+    assert m.seq[2](t) is t and torch.equal(t, blocks.dropout(x, 0.25, state.tensor, call=2))
+    t = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(m.seq[2](t * 1.0), [t], [torch.ones_like(t)])
+    assert torch.equal(g, blocks.dropout(x, 0.25, state.tensor, call=3))
+    other = copy.deepcopy(m)
+    assert type(other.a) is blocks.Dropout and other.a is other.b
+    blocks.use_in_training(m, None)
+    assert type(m.a) is type(m.seq[2]) is nn.Dropout and m.seq[2].inplace and type(m.own) is blocks.Dropout and m.own.state is None
+    torch.manual_seed(1)
+    want = torch.nn.functional.dropout(x, 0.5, True)
+    torch.manual_seed(1)
+    assert torch.equal(m.a(x), want) and len(seen) == 3
+    # again, another state in between; a dropout that is the whole model
+    second = blocks.DropoutState(4, device=device)
+    assert blocks.use_in_training(blocks.use_in_training(m, state), second).a.state is second and type(blocks.use_in_training(m, None).a) is nn.Dropout
+    bare = nn.Dropout(0.5)
+    assert blocks.use_in_training(bare, second) is bare and torch.equal(bare(x), blocks.dropout(x, 0.5, second.tensor, call=0))
+    assert type(blocks.use_in_training(bare, None)) is nn.Dropout

@@ -250,3 +250,7 @@ def test_forward_mode_is_refused():
 
 def test_tracers_and_wrapped_tensors_are_refused():
     bc.run_tracers_and_wrapped_tensors("cpu")
+
+
+def test_converted_dropouts():
+    bc.run_converted_dropouts("cpu")
