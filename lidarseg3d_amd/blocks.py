@@ -237,11 +237,16 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
 
 
 # ---------------------------------------------------------------------------------------------- the models' training forward
+def training_state(module):
+    """the DropoutState that use_in_training gave a module of this package; None in evaluation, also where evaluation is differentiated"""
+    return module.block_state if module.training else None
+
+
 def use_in_training(model, state):
     """Puts the training forward of a model of this package on the operators above: the SF-Phase decoder's and the TransVFE layers' residuals, dropouts and
     norms in one pass each, dropout (the decoder's and the heads' nn.Dropout) from `state`, a DropoutState, and the camera features' sampling on one
     weighted lookup.  The masks differ from torch's generator's (which still draws the class tokens' attention dropout inside nn.MultiheadAttention), everything
-    else agrees to rounding; evaluation is not touched.  The training loop
+    else agrees to rounding; a module in evaluation mode is not touched, with gradients or without.  The training loop
     calls state.advance() after each backward pass.  state None: back to the torch composition.  -> model"""
     if state is not None and not isinstance(state, DropoutState):
         raise TypeError("use_in_training: a DropoutState or None needed, got %s" % type(state).__name__)

@@ -541,15 +541,16 @@ def _sffm_forward_train(self, x, emb1, emb2, batch_idx, batch_size, return_conte
     mem = torch.cat([self.input_proj_embeddings1(emb1.squeeze(-1)), self.input_proj_embeddings2(emb2.squeeze(-1))], dim=2)
     mem = mem.permute(2, 0, 1).contiguous()  # [L, B, E]
     L = mem.shape[0]
+    state = blocks.training_state(self)
     for l in self.decoder.layers:
         p = l.dropout_p if self.training else 0.0
-        if self.block_state is None:
+        if state is None:
             drop = lambda t: F.dropout(t, p, self.training)
             join = lambda t, x, norm: norm(t + drop(x))
             act = lambda t: drop(F.relu(t))
         else:  # dropout, residual and norm in one pass each (blocks.use_in_training)
-            join = lambda t, x, norm: blocks.residual_norm(x, t, norm=blocks.Norm.of(norm), p=p, state=self.block_state)
-            act = lambda t: blocks.dropout(t, p, self.block_state, relu=True)
+            join = lambda t, x, norm: blocks.residual_norm(x, t, norm=blocks.Norm.of(norm), p=p, state=state)
+            act = lambda t: blocks.dropout(t, p, state, relu=True)
         mem = join(mem, l.self_attn(mem, mem, value=mem)[0], l.norm1)
         ca = l.crossocr_attn
         q = ca.q_proj(tgt).view(-1, H, hd)
@@ -687,7 +688,7 @@ class PointSegMSeg3DHead(PackedModule):
         pl = self.gffm_lidar(_interpolate_train(vf, idx, w, points, vx_off))
         cuv = batch_dict["points_cuv"]
         valid = cuv[:, 0] == 1
-        pc = self.gffm_camera(_sample_image_rows(batch_dict["image_features"], cuv[valid], points[:, 0][valid], self.block_state is not None))
+        pc = self.gffm_camera(_sample_image_rows(batch_dict["image_features"], cuv[valid], points[:, 0][valid], blocks.training_state(self) is not None))
         ppc = self.lidar_camera_mimic_layer(pl[valid])
         # completed camera features (:320-334): rows without a camera hit stay zero, the pseudo-camera branch only
         # exists on the rows WITH a hit and feeds nothing but the mimic loss

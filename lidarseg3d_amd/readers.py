@@ -137,7 +137,7 @@ class TransformerVoxelFeatureExtractor(PackedModule):
         tok = ops.vfe_tokens(features.contiguous(), num_voxels.to(torch.int32).contiguous(), (kt + 15) // 16 * 16)[:, :kt]
         conv = self.feature_conv[0]
         x = torch.nn.functional.linear(tok, conv.weight.squeeze(-1), conv.bias).view(V, P, self.num_embed).permute(1, 0, 2)
-        if self.block_state is None or not len(self.chunck.layers):
+        if blocks.training_state(self) is None or not len(self.chunck.layers):
             for l in self.chunck.layers:  # voxel_encoder.py:149-163: the residuals start from the NORMED tensor
                 x = l.norm1(x)
                 x = x + l.self_attn(x, x, x, need_weights=False)[0]

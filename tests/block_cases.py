@@ -783,3 +783,44 @@ def run_converted_dropouts(device):
     bare = nn.Dropout(0.5)
     assert blocks.use_in_training(bare, second) is bare and torch.equal(bare(x), blocks.dropout(x, 0.5, second.tensor, call=0))
     assert type(blocks.use_in_training(bare, None)) is nn.Dropout
+
+
+def run_differentiated_evaluation(device, points):
+    """modules in evaluation mode compute the torch composition bit for bit after use_in_training, gradients included"""
+    from lidarseg3d_amd import blocks, point_heads, readers
+    torch.manual_seed(6)
+    gen = torch.Generator().manual_seed(7)
+    decoder = point_heads.SemanticFeatureFusionModule(64, 48, 32, d_model=96, nhead=4, num_decoder_layers=1, dim_feedforward=192, dropout=0.3).to(device).eval()
+    reader = readers.TransformerVoxelFeatureExtractor(num_input_features=5, num_layers=1).to(device).eval()
+    x = tensor(gen, points, 64, device=device).requires_grad_()
+    e1, e2 = tensor(gen, 2, 48, 9, 1, device=device), tensor(gen, 2, 32, 9, 1, device=device)
+    batch = (torch.arange(points) * 2 // points).float().to(device)
+    vox, num = tensor(gen, points, 5, 5, device=device), (torch.arange(points) % 5 + 1).to(torch.int32).to(device)
+    forms = {"decoder": (decoder, lambda m: m._forward_train(x, e1, e2, batch, 2), [x] + list(decoder.parameters())),
+             "reader": (reader, lambda m: m._forward_train(vox, num), list(reader.parameters()))}
+    state = blocks.DropoutState(1, device=device)
+    calls = []
+    keep = blocks.residual_norm
+    blocks.residual_norm = lambda *a, **k: (calls.append(1), keep(*a, **k))[1]
+    try:
+        for name, (m, f, leaves) in forms.items():
+            res = []
+            for s in (None, state):
+                y = f(blocks.use_in_training(m, s))
+                res.append([y.detach()] + list(torch.autograd.grad(y, leaves, [torch.ones_like(y)], allow_unused=True)))
+                assert not calls, name
+            if device == "cpu":  # (on the device a library product may add in another order; the operators are not called at all there, above)
+                assert torch.equal(res[0][0], res[1][0]), name
+            m.train()
+            f(m)
+            assert calls, name
+            calls.clear()
+            m.eval()
+    finally:
+        blocks.residual_norm = keep
+    head = point_heads.PointSegMSeg3DHead
+    assert head.block_state is None
+    stub = type("M", (), {"block_state": state, "training": False})()
+    assert blocks.training_state(stub) is None
+    stub.training = True
+    assert blocks.training_state(stub) is state and state.calls > 0

@@ -245,3 +245,7 @@ def test_tracers_and_wrapped_tensors_are_refused():
 
 def test_converted_dropouts():
     bc.run_converted_dropouts(DEV)
+
+
+def test_differentiated_evaluation():
+    bc.run_differentiated_evaluation(DEV, 700)

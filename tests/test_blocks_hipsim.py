@@ -254,3 +254,7 @@ def test_tracers_and_wrapped_tensors_are_refused():
 
 def test_converted_dropouts():
     bc.run_converted_dropouts("cpu")
+
+
+def test_differentiated_evaluation():
+    bc.run_differentiated_evaluation("cpu", 23)
