@@ -83,6 +83,14 @@ struct ls3d_rn_map {
       ls3d_param4(p, dtype, first(lane, i) + LPR * 4, c, otherwise, v + 4);
     } else ls3d_param8(p, dtype, first(lane, i), c, otherwise, v);
   }
+  // bits of the m live columns of a chunk; the others count as dropped: a norm before leaves NaN there in a row that holds infinities, and a row of which
+  // the mask leaves nothing must not see them
+  static __device__ __forceinline__ uint32_t live(uint32_t keep, int m) {
+    if constexpr (SPLIT) {
+      const int b = m - LPR * 4;
+      return keep & ((m >= 4 ? 15u : (1u << (m > 0 ? m : 0)) - 1u) | (b >= 4 ? 15u : (1u << (b > 0 ? b : 0)) - 1u) << 4);
+    } else return m >= 8 ? keep : keep & ((1u << (m > 0 ? m : 0)) - 1u);
+  }
   static __device__ __forceinline__ uint32_t keep(const ls3d_dropout_key &key, int lane, int i, uint32_t row, uint32_t thr) {
     if constexpr (SPLIT) {  // halves of two counters
       const uint32_t a = (uint32_t)first(lane, i), b = a + LPR * 4;
@@ -219,7 +227,8 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>()) void k_resnorm_fwd(const ls
     if (A.thr) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        const uint32_t keep = M::keep(key, lane, i, (uint32_t)row, A.thr);
+        uint32_t keep = M::keep(key, lane, i, (uint32_t)row, A.thr);
+        if (FULL) keep = M::live(keep, m0 - i * LPR * 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = ((keep >> j) & 1u) ? v[i][j] * A.inv : 0.0f;
       }
@@ -329,6 +338,7 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_r
       keep[i] = 0xFFu;
       if (A.thr) {
         keep[i] = M::keep(key, lane, i, (uint32_t)row, A.thr);
+        if (FULL) keep[i] = M::live(keep[i], m0 - i * LPR * 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sh[i][j] = ((keep[i] >> j) & 1u) ? sh[i][j] * A.inv : 0.0f;
       }

@@ -824,3 +824,33 @@ def run_differentiated_evaluation(device, points):
     assert blocks.training_state(stub) is None
     stub.training = True
     assert blocks.training_state(stub) is state and state.calls > 0
+
+
+def run_dropped_rows_beside_infinities(device):
+    """rows of infinities and NaN behind a norm, of which the mask leaves nothing, at widths that leave lanes without columns: such a row is its residual, its norm and
+    the residual's gradient are those of a row of zeros"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(41)
+    for c, p, T, R, gate_kind in ((1, 0.9, F32, F32, None), (7, 0.9, BF16, BF16, "channel"), (9, 0.9, F16, F32, None), (70, 0.99, F32, F32, "full"), (70, 0.99, BF16, F32, None),
+                                  (100, 0.99, F32, F32, None), (523, 0.999, F32, F32, "channel"), (523, 0.999, F16, F16, None)):
+        n = 60
+        for kind in ("layer", "rms"):
+            x = torch.full((n, c), float("inf"), dtype=T)
+            x[::3, c // 2] = float("nan")
+            x[1::3] = -x[1::3]
+            r, dy = tensor(gen, n, c, dtype=R), tensor(gen, n, c, dtype=T)
+            gate = {None: None, "channel": tensor(gen, c), "full": tensor(gen, n, c, dtype=T)}[gate_kind]
+            norm_in, norm = (kind, tensor(gen, c), tensor(gen, c), 1e-5), ("layer", tensor(gen, c), None, 1e-5)
+            keep, _ = keep_mask(n, c, p, 8, 0, 4)
+            gone = ~keep.any(1)
+            assert 5 <= int(gone.sum()) < n, (c, int(gone.sum()))
+            put = lambda t: None if t is None else t.to(device)
+            xd, rd = put(x).requires_grad_(), put(r).requires_grad_()
+            mod = lambda m: blocks.Norm(m[0], put(m[1]), put(m[2]), m[3])
+            y, s = blocks.residual_norm(xd, rd, norm=mod(norm), norm_in=mod(norm_in), gate=put(gate), alpha=0.5, p=p, state=blocks.DropoutState(8, device=device).tensor, call=4,
+                                        return_sum=True)
+            (dr,) = torch.autograd.grad(y, [rd], [put(dy)])
+            ref = residual_norm_reference(torch.zeros_like(x), r, norm, norm_in, gate, 0.5, p, (8, 0, 4), dy, None)
+            for name, got in (("y", y), ("s", s), ("residual", dr)):
+                value, scale = ref[name]
+                check(got.detach().cpu()[gone], value[gone], scale[gone], what="%s, c %d, %s" % (name, c, kind))

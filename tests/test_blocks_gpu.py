@@ -249,3 +249,7 @@ def test_converted_dropouts():
 
 def test_differentiated_evaluation():
     bc.run_differentiated_evaluation(DEV, 700)
+
+
+def test_dropped_rows_beside_infinities():
+    bc.run_dropped_rows_beside_infinities(DEV)
