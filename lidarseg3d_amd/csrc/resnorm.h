@@ -83,13 +83,13 @@ struct ls3d_rn_map {
       ls3d_param4(p, dtype, first(lane, i) + LPR * 4, c, otherwise, v + 4);
     } else ls3d_param8(p, dtype, first(lane, i), c, otherwise, v);
   }
-  // bits of the m live columns of a chunk; the others count as dropped: a norm before leaves NaN there in a row that holds infinities, and a row of which
-  // the mask leaves nothing must not see them
-  static __device__ __forceinline__ uint32_t live(uint32_t keep, int m) {
-    if constexpr (SPLIT) {
-      const int b = m - LPR * 4;
-      return keep & ((m >= 4 ? 15u : (1u << (m > 0 ? m : 0)) - 1u) | (b >= 4 ? 15u : (1u << (b > 0 ? b : 0)) - 1u) << 4);
-    } else return m >= 8 ? keep : keep & ((1u << (m > 0 ? m : 0)) - 1u);
+  // zeros behind the row's end, m live columns: what a norm makes of the zeros there, (0 - mean) / std, is infinite for a mean near the largest values and NaN for a
+  // row that holds infinities, and even a product with zero would carry that into the row's sums
+  static __device__ __forceinline__ void clip(float (&v)[8], int m) {
+    if (m >= (SPLIT ? LPR * 4 + 4 : 8)) return;
+    LS3D_OPAQUE(m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (SPLIT && j >= 4 ? LPR * 4 + j - 4 : j) < m ? v[j] : 0.0f;
   }
   static __device__ __forceinline__ uint32_t keep(const ls3d_dropout_key &key, int lane, int i, uint32_t row, uint32_t thr) {
     if constexpr (SPLIT) {  // halves of two counters
@@ -220,15 +220,16 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>()) void k_resnorm_fwd(const ls
     if (FULL && A.kind_in) {
       ls3d_rn_stats<LPR, VPT, SPLIT>(v, A.kind_in, m0, inv_c, A.eps_in, sums, st[0], st[1]);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
+      for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - st[0]) * st[1], wi[i][j], bi[i][j]);  // (behind the end: weight and bias are zero)
+        for (int j = 0; j < 8; ++j) v[i][j] = fmaf((v[i][j] - st[0]) * st[1], wi[i][j], bi[i][j]);
+        M::clip(v[i], m0 - i * LPR * 8);
+      }
     }
     if (A.thr) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        uint32_t keep = M::keep(key, lane, i, (uint32_t)row, A.thr);
-        if (FULL) keep = M::live(keep, m0 - i * LPR * 8);
+        const uint32_t keep = M::keep(key, lane, i, (uint32_t)row, A.thr);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = ((keep >> j) & 1u) ? v[i][j] * A.inv : 0.0f;
       }
@@ -330,15 +331,14 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_r
       M::template unpack<TX>(rx[i], m0 - i * LPR * 8, sh[i]);
       if (FULL) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          xh[i][j] = A.kind_in ? (sh[i][j] - st.x) * st.y : sh[i][j];
-          sh[i][j] = A.kind_in ? fmaf(xh[i][j], wi[i][j], bi[i][j]) : xh[i][j];
-        }
+        for (int j = 0; j < 8; ++j) xh[i][j] = A.kind_in ? (sh[i][j] - st.x) * st.y : sh[i][j];
+        M::clip(xh[i], m0 - i * LPR * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sh[i][j] = A.kind_in ? fmaf(xh[i][j], wi[i][j], bi[i][j]) : xh[i][j];
       }
       keep[i] = 0xFFu;
       if (A.thr) {
         keep[i] = M::keep(key, lane, i, (uint32_t)row, A.thr);
-        if (FULL) keep[i] = M::live(keep[i], m0 - i * LPR * 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sh[i][j] = ((keep[i] >> j) & 1u) ? sh[i][j] * A.inv : 0.0f;
       }
@@ -361,8 +361,10 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>(), LPR > 512 ? 4 : 2) void k_r
       for (int i = 0; i < VPT; ++i) {
         M::template unpack<TX>(ry[i], m0 - i * LPR * 8, S[i]);  // zeros behind the row's end keep what stands there out of every sum
 #pragma unroll
+        for (int j = 0; j < 8; ++j) sh[i][j] = (sh[i][j] - st.z) * st.w;
+        M::clip(sh[i], m0 - i * LPR * 8);
+#pragma unroll
         for (int j = 0; j < 8; ++j) {
-          sh[i][j] = (sh[i][j] - st.z) * st.w;
           acc[0][i][j] = fmaf(S[i][j], sh[i][j], acc[0][i][j]);
           acc[1][i][j] += S[i][j];
           S[i][j] *= wo[i][j];

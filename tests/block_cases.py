@@ -854,3 +854,36 @@ def run_dropped_rows_beside_infinities(device):
             for name, got in (("y", y), ("s", s), ("residual", dr)):
                 value, scale = ref[name]
                 check(got.detach().cpu()[gone], value[gone], scale[gone], what="%s, c %d, %s" % (name, c, kind))
+
+
+def run_rows_near_the_largest_value(device):
+    """equal values near the type's largest at widths that leave lanes without columns: (0 - mean) / std overflows there and must not reach the row, its gradient or, through rows
+    that a workgroup does not have, the parameters' gradients.  Values and widths are powers of two: mean and deviation are exact"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(43)
+    n, eps = 5, 1e-5
+    std = eps ** -0.5
+    for T in (F32, BF16):
+        for c in (1, 2, 4, 8, 16):
+            x = torch.full((n, c), -2.0 ** 127, dtype=T, device=device).requires_grad_()
+            w, b = (tensor(gen, c, device=device).requires_grad_() for _ in range(2))
+            wi = tensor(gen, c, device=device).requires_grad_()
+            dy = tensor(gen, n, c, dtype=T, device=device)
+            # norm alone: y = b, dx = (u - mean u) / std with u = w dy, dw = 0, db = sum dy
+            y = blocks.residual_norm(x, norm=blocks.Norm("layer", w, b, eps))
+            dx, dw, db = torch.autograd.grad(y, [x, w, b], [dy])
+            dyd = dy.cpu().double()
+            u = dyd * w.detach().cpu().double()
+            check(y, b.detach().cpu().double().expand(n, c), 0.0, what="y")
+            check(dx, std * (u - u.mean(1, keepdim=True)), std * _rmax(u), what="dx")
+            assert bool((dw == 0).all()), (T, c)
+            check(db, dyd.sum(0), dyd.abs().sum(0), what="db")
+            # behind another norm: t = 0, s = residual
+            r = tensor(gen, n, c, dtype=T, device=device).requires_grad_()
+            y, s = blocks.residual_norm(x, r, norm=blocks.Norm("rms", w, None, eps), norm_in=blocks.Norm("layer", wi, None, eps), return_sum=True)
+            gx, gr, gw, gi = torch.autograd.grad([y, s], [x, r, w, wi], [dy, dy])
+            assert torch.equal(s, r) and torch.isfinite(gx).all() and bool((gi == 0).all()), (T, c)
+            ref = residual_norm_reference(torch.zeros(n, c), r, ("rms", w, None, eps), ("layer", wi, None, eps), None, 1.0, 0.0, None, dy, dy)
+            check(y, *ref["y"], what="y behind a norm")
+            check(gr, *ref["residual"], what="d residual")
+            check(gw, *ref["w_out"], what="d weight")

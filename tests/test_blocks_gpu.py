@@ -253,3 +253,7 @@ def test_differentiated_evaluation():
 
 def test_dropped_rows_beside_infinities():
     bc.run_dropped_rows_beside_infinities(DEV)
+
+
+def test_rows_near_the_largest_value():
+    bc.run_rows_near_the_largest_value(DEV)

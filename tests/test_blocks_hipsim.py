@@ -262,3 +262,7 @@ def test_differentiated_evaluation():
 
 def test_dropped_rows_beside_infinities():
     bc.run_dropped_rows_beside_infinities("cpu")
+
+
+def test_rows_near_the_largest_value():
+    bc.run_rows_near_the_largest_value("cpu")
