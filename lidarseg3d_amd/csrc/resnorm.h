@@ -25,6 +25,7 @@ struct ls3d_rn_args {
   const void *w_in, *b_in, *w_out, *b_out;
   int w_in_t, b_in_t, w_out_t, b_out_t, gate_t;
   float eps_in, eps_out, alpha, inv;
+  float share, whole;  // a row's mean: the sum of share * value divided by whole; share: a power of two, whole: c * share in (0.5, 1]
   uint32_t thr, call;
   const int64_t *state;
   float *stats;  // [n][4]: mean, rstd of N_in, mean, rstd of N_out
@@ -136,18 +137,21 @@ struct ls3d_row_sums {
 };
 
 // mean and 1 / sqrt(variance + eps) of a row's values (two passes over registers: no cancellation); RMS: mean 0.  Columns behind the row's end hold zeros;
-// m0: live columns from the lane's first chunk on
+// m0: live columns from the lane's first chunk on.  The mean is summed in shares, so that a row of the type's lowest values does not overflow, and a share is
+// exact: equal values of 2-byte types then have their value as mean and deviation 0 at any c (in shares of 1 / c each is rounded: 60000 at c = 96 is off by 0.01
+// alike in every column, which the norm makes +-1 of).  Cost: a division a row.
 template <int LPR, int VPT, bool SPLIT>
-__device__ __forceinline__ void ls3d_rn_stats(const float (&v)[VPT][8], int kind, int m0, float inv_c, float eps, ls3d_row_sums<LPR> &sums, float &mean, float &rstd) {
+__device__ __forceinline__ void ls3d_rn_stats(const float (&v)[VPT][8], int kind, int m0, const ls3d_rn_args &A, float inv_c, float eps, ls3d_row_sums<LPR> &sums,
+                                              float &mean, float &rstd) {
   mean = 0.0f;
   if (kind == LS3D_NORM_LAYER) {
     float a = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a = fmaf(v[i][j], inv_c, a);  // shares of the mean: a row of the type's lowest values does not overflow
+      for (int j = 0; j < 8; ++j) a = fmaf(v[i][j], A.share, a);
     sums(a);
-    mean = a;
+    mean = a / A.whole;
   }
   float q = 0.0f;
 #pragma unroll
@@ -218,7 +222,7 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>()) void k_resnorm_fwd(const ls
     for (int i = 0; i < VPT; ++i) M::template unpack<TX>(rx[i], m0 - i * LPR * 8, v[i]);
     float st[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (FULL && A.kind_in) {
-      ls3d_rn_stats<LPR, VPT, SPLIT>(v, A.kind_in, m0, inv_c, A.eps_in, sums, st[0], st[1]);
+      ls3d_rn_stats<LPR, VPT, SPLIT>(v, A.kind_in, m0, A, inv_c, A.eps_in, sums, st[0], st[1]);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
 #pragma unroll
@@ -256,7 +260,7 @@ __global__ __launch_bounds__(ls3d_rn_threads<LPR>()) void k_resnorm_fwd(const ls
       for (int i = 0; i < VPT; ++i) M::template store<TR, NT>(A.s, row, lane, i, c, v[i], m0 - i * LPR * 8);
     }
     if (A.kind_out) {
-      ls3d_rn_stats<LPR, VPT, SPLIT>(v, A.kind_out, m0, inv_c, A.eps_out, sums, st[2], st[3]);
+      ls3d_rn_stats<LPR, VPT, SPLIT>(v, A.kind_out, m0, A, inv_c, A.eps_out, sums, st[2], st[3]);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         float o[8];

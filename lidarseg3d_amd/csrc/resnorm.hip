@@ -76,6 +76,9 @@ static int rn_fill(const ls3d_residual_norm_t *d, const void *x, long long x_ld,
   a->n = n; a->c = c;
   a->kind_in = d->in.kind; a->w_in = d->in.weight; a->b_in = d->in.bias; a->w_in_t = d->in.weight_dtype; a->b_in_t = d->in.bias_dtype; a->eps_in = d->in.eps;
   a->kind_out = d->out.kind; a->w_out = d->out.weight; a->b_out = d->out.bias; a->w_out_t = d->out.weight_dtype; a->b_out_t = d->out.bias_dtype; a->eps_out = d->out.eps;
+  a->share = 1.0f;
+  while ((float)c * a->share > 1.0f) a->share *= 0.5f;
+  a->whole = (float)c * a->share;
   a->alpha = d->alpha; a->state = d->state; a->call = d->call;
   return LS3D_OK;
 }

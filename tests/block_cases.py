@@ -887,3 +887,25 @@ def run_rows_near_the_largest_value(device):
             check(y, *ref["y"], what="y behind a norm")
             check(gr, *ref["residual"], what="d residual")
             check(gw, *ref["w_out"], what="d weight")
+
+
+def run_rows_of_equal_values(device):
+    """rows of one value at widths that are no power of two: 2-byte values times up to 8192 add up exactly in 32 bits, so the deviation is 0, the norm is its bias and the
+    gradient of its weight is 0; the type's lowest and highest values do not overflow on the way"""
+    from lidarseg3d_amd import blocks
+    for T in (BF16, F16, F32):
+        for c in (1, 3, 17, 65, 96, 129, 517, 771, 1000, 4099, 8191):
+            top = float(torch.finfo(T).max)
+            values = torch.tensor([top, -top, 60000.0, 0.1, -0.1, 1.0 / 3.0, 0.0, float(torch.finfo(T).tiny)]).to(T if T != F32 else BF16).to(T)  # (f32: values of 8 bits, and its extremes)
+            if T == F32:
+                values[0], values[1] = 2.0 ** 127, -2.0 ** 127
+            x = values.unsqueeze(1).expand(-1, c).contiguous().to(device)
+            w, b = torch.full((c,), 2.0, device=device, requires_grad=True), torch.arange(float(c), device=device)
+            for norm_in in (None, blocks.Norm("layer")):
+                y = blocks.residual_norm(x, norm=blocks.Norm("layer", w, b.to(T)), norm_in=norm_in)
+                assert torch.equal(y.detach(), b.to(T).expand_as(y)), (T, c)
+                (dw,) = torch.autograd.grad(y, [w], [torch.ones_like(y)])
+                assert bool((dw == 0).all()), (T, c)
+    # a residual that leaves one value in every column
+    x, r = torch.full((5, 771), 512.0, dtype=F16, device=device), torch.full((5, 771), 7.0, dtype=F16, device=device)
+    assert bool((blocks.residual_norm(x, r, norm=blocks.Norm("layer"), alpha=-3.0) == 0).all())

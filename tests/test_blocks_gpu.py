@@ -257,3 +257,7 @@ def test_dropped_rows_beside_infinities():
 
 def test_rows_near_the_largest_value():
     bc.run_rows_near_the_largest_value(DEV)
+
+
+def test_rows_of_equal_values():
+    bc.run_rows_of_equal_values(DEV)
