@@ -188,7 +188,7 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
             if gate.dtype != x.dtype:
                 raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
         elif gate.numel() == 1 or gate.shape == (c,):
-            gate = gate if gate.shape == (c,) else gate.reshape(1).expand(c)
+            gate = gate if gate.shape == (c,) else gate.reshape(1).float().expand(c)  # (float: its gradient is the sum of c channels', rounded once at the end)
             if not gate.is_contiguous():
                 gate = gate.contiguous()
         else:

@@ -261,3 +261,7 @@ def test_rows_near_the_largest_value():
 
 def test_rows_of_equal_values():
     bc.run_rows_of_equal_values(DEV)
+
+
+def test_single_value_gates():
+    bc.run_single_value_gates(DEV)

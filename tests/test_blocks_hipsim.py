@@ -270,3 +270,7 @@ def test_rows_near_the_largest_value():
 
 def test_rows_of_equal_values():
     bc.run_rows_of_equal_values("cpu")
+
+
+def test_single_value_gates():
+    bc.run_single_value_gates("cpu")
