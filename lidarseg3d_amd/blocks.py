@@ -184,7 +184,7 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
             raise TypeError("residual: %s or float32 needed, got %s" % (x.dtype, residual.dtype))
     if gate is not None:
         _dtype_ok(gate, "gate")
-        if gate.shape == shape and gate.dim() > 1:
+        if gate.shape == shape and gate.dim() > 1 and gate.numel() != 1:
             if gate.dtype != x.dtype:
                 raise TypeError("a gate for each element has x's type (%s), got %s" % (x.dtype, gate.dtype))
         elif gate.numel() == 1 or gate.shape == (c,):

@@ -925,3 +925,13 @@ def run_single_value_gates(device):
             assert torch.equal(s, 0.5 * x.to(R))
             (dg,) = torch.autograd.grad(s, [g], [torch.ones(2, c, dtype=R, device=device)])
             assert dg.shape == g.shape and dg.dtype == T and float(dg) == want, (T, shape, float(dg))
+
+
+def run_one_element_with_a_gate(device):
+    """x of one element and a gate of one element in another type: a single value, as at any other size"""
+    from lidarseg3d_amd import blocks
+    for shape in ((1, 1), (1, 1, 1)):
+        x, g = torch.full(shape, 3.0, dtype=BF16, device=device, requires_grad=True), torch.full(shape, 0.5, device=device, requires_grad=True)
+        y = blocks.residual_norm(x, gate=g)
+        dx, dg = torch.autograd.grad(y, [x, g], [torch.full(shape, 2.0, dtype=BF16, device=device)])
+        assert float(y) == 1.5 and float(dx) == 1.0 and float(dg) == 6.0 and y.shape == dx.shape == dg.shape == shape

@@ -265,3 +265,7 @@ def test_rows_of_equal_values():
 
 def test_single_value_gates():
     bc.run_single_value_gates(DEV)
+
+
+def test_one_element_with_a_gate():
+    bc.run_one_element_with_a_gate(DEV)
