@@ -86,6 +86,11 @@ def _on_device(t, what):
         raise RuntimeError("%s: lidarseg3d_amd ops need tensors on the MI355X (got a %s tensor); there is no CPU fallback" % (what, t.device))
 
 
+def _number(v, what):
+    if torch.is_tensor(v) and v.requires_grad:
+        raise TypeError("%s is a number: a tensor that requires a gradient would not get one" % what)
+
+
 def _draw(p, state, call):
     """-> (p, state tensor, call) of a dropout"""
     if p == 0.0:
@@ -193,6 +198,7 @@ def residual_norm(x, residual=None, norm=None, norm_in=None, gate=None, alpha=1.
                 gate = gate.contiguous()
         else:
             raise ValueError("gate %s: one value, [%d] or %s" % (tuple(gate.shape), c, tuple(shape)))
+    _number(alpha, "alpha")
     w_in, b_in, kind_in, eps_in = _NO_NORM if norm_in is None else _norm_arguments(norm_in, c, "norm_in")
     w_out, b_out, kind_out, eps_out = _NO_NORM if norm is None else _norm_arguments(norm, c, "norm")
     p, state, call = _draw(p, state, call)
@@ -222,6 +228,7 @@ def embedding(table, idx, weight=None, scale=1.0, padding_idx=None, bag=False):
         bag = True
     if bag and (idx.dim() < 1 or idx.shape[-1] == 0):
         raise ValueError("embedding: no indices to sum over")
+    _number(scale, "scale")
     if padding_idx is not None and not -table.shape[0] <= padding_idx < table.shape[0]:
         raise ValueError("padding_idx %r outside a table of %d rows" % (padding_idx, table.shape[0]))
     padding = -1 if padding_idx is None else int(padding_idx) % table.shape[0]

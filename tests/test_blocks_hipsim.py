@@ -278,3 +278,14 @@ def test_single_value_gates():
 
 def test_one_element_with_a_gate():
     bc.run_one_element_with_a_gate("cpu")
+
+
+def test_learned_numbers_are_refused():
+    """alpha and scale are numbers: as learned tensors they would be read and never get a gradient; tensors that want none are read"""
+    x, table, ix = torch.ones(2, 4), torch.ones(3, 4), torch.tensor([0, 2])
+    for learned in (torch.tensor(2.0, requires_grad=True), torch.nn.Parameter(torch.ones(1))):
+        with pytest.raises(TypeError, match="alpha is a number"):
+            blocks.residual_norm(x, x, alpha=learned)
+        with pytest.raises(TypeError, match="scale is a number"):
+            blocks.embedding(table, ix, scale=learned)
+    assert bool((blocks.residual_norm(x, x, alpha=torch.tensor(2.0)) == 3).all()) and bool((blocks.embedding(table, ix, scale=torch.tensor(2.0)) == 2).all())
