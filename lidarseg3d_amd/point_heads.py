@@ -576,9 +576,12 @@ SemanticFeatureFusionModule._forward_train = _sffm_forward_train
 def _sample_image_rows(image_features, cuv, batch_idx, lookup=False):
     """get_points_image_feature (point_seg_mseg3d_head.py:200-236) under autograd: the 5-D bilinear grid_sample
     (align_corners=True, zeros padding) written as 8 weighted row gathers from the channels-last maps, all frames at once;
-    lookup: as one weighted row lookup (blocks.embedding), the maps' gradient sorted and added in a fixed order instead of eight scatters"""
+    lookup: as one weighted row lookup (blocks.embedding, f32 weights; wider coordinates or maps keep the gathers), the maps' gradient sorted and added in a fixed
+    order instead of eight scatters"""
     B, ncam, C, h, w = image_features.shape
     rows = image_features.permute(0, 1, 3, 4, 2).reshape(-1, C)
+    wide = torch.promote_types(rows.dtype, cuv.dtype)  # what the products with the weights are formed and returned in
+    lookup = lookup and wide == torch.float32
     pos = [(cuv[:, 1] + 1) * 0.5 * (ncam - 1), (cuv[:, 2] + 1) * 0.5 * (h - 1), (cuv[:, 3] + 1) * 0.5 * (w - 1)]
     lim = [ncam, h, w]
     lo = [p.floor() for p in pos]
@@ -597,7 +600,7 @@ def _sample_image_rows(image_features, cuv, batch_idx, lookup=False):
             weights.append(wgt)
         else:
             out = out + rows[flat] * (wgt * inside).unsqueeze(1)
-    return blocks.embedding(rows, torch.stack(entries, 1), weight=torch.stack(weights, 1)) if lookup else out
+    return blocks.embedding(rows.to(wide), torch.stack(entries, 1), weight=torch.stack(weights, 1).to(wide)) if lookup else out
 
 
 @POINT_HEADS.register_module

@@ -934,4 +934,26 @@ def run_one_element_with_a_gate(device):
         x, g = torch.full(shape, 3.0, dtype=BF16, device=device, requires_grad=True), torch.full(shape, 0.5, device=device, requires_grad=True)
         y = blocks.residual_norm(x, gate=g)
         dx, dg = torch.autograd.grad(y, [x, g], [torch.full(shape, 2.0, dtype=BF16, device=device)])
-        assert float(y) == 1.5 and float(dx) == 1.0 and float(dg) == 6.0 and y.shape == dx.shape == dg.shape == shape
+        assert float(y.detach()) == 1.5 and float(dx) == 1.0 and float(dg) == 6.0 and y.shape == dx.shape == dg.shape == shape
+
+
+def run_camera_sampling_types(device):
+    """camera maps of a 2-byte type (an image network in mixed precision) and of float64, coordinates of either: the lookup gives what the gathers give, in their type"""
+    from lidarseg3d_amd import point_heads
+    gen = torch.Generator().manual_seed(61)
+    points = 50
+    cuv = torch.cat([torch.ones(points, 1), torch.randint(0, 2, (points, 1), generator=gen).float() * 2 - 1.0, torch.rand(points, 2, generator=gen) * 2.4 - 1.2], 1).to(device)
+    bidx = torch.zeros(points, device=device)
+    for T, P in ((BF16, F32), (F16, F32), (F32, F32), (torch.float64, F32), (F32, torch.float64), (F32, F16), (F16, F16)):
+        img = tensor(gen, 1, 2, 16, 5, 7, device=device).to(T).requires_grad_()
+        want, got = (point_heads._sample_image_rows(img, cuv.to(P), bidx, lookup) for lookup in (False, True))
+        assert got.dtype == want.dtype, (T, P)
+        # eight products, added in the same order; a 2-byte sum of the gathers is rounded at every step
+        assert float((got.double() - want.double()).abs().max()) <= (16 * unit(want.dtype) + K32) * float(img.detach().abs().max()), (T, P)
+        dy = tensor(gen, points, 16, device=device).to(want.dtype)
+        (g,) = torch.autograd.grad(got, [img], [dy])
+        assert g.dtype == T, (T, P)
+        if want.dtype == F32:  # the lookup: sums in 32 bits, rounded to the maps' type once; the gathers in float64 with the same weights as reference
+            i64 = img.detach().cpu().double().requires_grad_()
+            ref, mag = (torch.autograd.grad(point_heads._sample_image_rows(i64, cuv.cpu().to(P), bidx.cpu()), [i64], [d])[0] for d in (dy.cpu().double(), dy.cpu().double().abs()))
+            check(g, ref, mag, what="d maps", k=(points + 16) * 2.0 ** -24)

@@ -269,3 +269,7 @@ def test_single_value_gates():
 
 def test_one_element_with_a_gate():
     bc.run_one_element_with_a_gate(DEV)
+
+
+def test_camera_sampling_types():
+    bc.run_camera_sampling_types(DEV)

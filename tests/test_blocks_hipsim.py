@@ -289,3 +289,7 @@ def test_learned_numbers_are_refused():
         with pytest.raises(TypeError, match="scale is a number"):
             blocks.embedding(table, ix, scale=learned)
     assert bool((blocks.residual_norm(x, x, alpha=torch.tensor(2.0)) == 3).all()) and bool((blocks.embedding(table, ix, scale=torch.tensor(2.0)) == 2).all())
+
+
+def test_camera_sampling_types():
+    bc.run_camera_sampling_types("cpu")
