@@ -60,8 +60,11 @@ int code(const Tensor &t) {
   TORCH_CHECK(s == at::kFloat || s == at::kBFloat16 || s == at::kHalf, "float32, bfloat16 or float16 needed");
   return s == at::kFloat ? LS3D_DTYPE_F32 : s == at::kBFloat16 ? LS3D_DTYPE_BF16 : LS3D_DTYPE_F16;
 }
+// the values themselves: memory may hold them with the other sign (the imaginary part of a conjugate)
+Tensor values(const Tensor &t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // [..., c] as rows the kernels take: a view where the rows are contiguous, else a copy
-Tensor rows(const Tensor &t) {
+Tensor rows(const Tensor &x) {
+  const Tensor t = values(x);
   const int64_t c = t.size(-1);
   Tensor r = t.dim() == 2 ? t : t.reshape({c ? t.numel() / c : 0, c});
   if (r.is_contiguous()) return r;
@@ -195,14 +198,14 @@ variable_list norm_outputs(const NormForm &f, const std::array<Tensor, 3> &o) {
   return {f.kind_out ? o[0] : o[1]};
 }
 
-Tensor gate_rows(const Tensor &g) { return g.defined() ? g.dim() == 1 ? g.contiguous() : rows(g) : Tensor(); }
+Tensor gate_rows(const Tensor &g) { return g.defined() ? g.dim() == 1 ? values(g).contiguous() : rows(g) : Tensor(); }
 
 // Takes the caller's tensors and makes rows of them inside: a gradient goes back as the one tensor that the kernel wrote.  Views of it, as a reshape before the
 // Function would make, look like tensors of their own to the engine, which then keeps and adds to each as if no other shared its memory.
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list forward(AutogradContext *ctx, const Tensor &x, const Optional &residual, const Optional &gate, const Optional &w_in, const Optional &b_in,
                                const Optional &w_out, const Optional &b_out, const Optional &state, const NormForm &f) {
-    const Tensor t[] = {rows(x), residual ? rows(*residual) : Tensor(), gate_rows(tensor(gate)), tensor(w_in), tensor(b_in), tensor(w_out), tensor(b_out), tensor(state)};
+    const Tensor t[] = {rows(x), residual ? rows(*residual) : Tensor(), gate_rows(tensor(gate)), values(tensor(w_in)), values(tensor(b_in)), values(tensor(w_out)), values(tensor(b_out)), tensor(state)};
     const auto o = norm_raw(f, x.sizes(), t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], true);
     ctx->save_for_backward({t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], o[2]});
     ctx->saved_data["f"] = f.pack();
@@ -255,7 +258,7 @@ variable_list residual_norm(const Tensor &x, const Optional &residual, const Opt
   bool grad = false;
   for (const Tensor &u : t) grad = grad || (u.defined() && u.requires_grad());
   if (grad && at::GradMode::is_enabled()) return ResidualNorm::apply(x, maybe(t[1]), maybe(t[2]), maybe(t[3]), maybe(t[4]), maybe(t[5]), maybe(t[6]), state, f);
-  return norm_outputs(f, norm_raw(f, x.sizes(), rows(x), t[1].defined() ? rows(t[1]) : Tensor(), gate_rows(t[2]), t[3], t[4], t[5], t[6], tensor(state), false));
+  return norm_outputs(f, norm_raw(f, x.sizes(), rows(x), t[1].defined() ? rows(t[1]) : Tensor(), gate_rows(t[2]), values(tensor(w_in)), values(tensor(b_in)), values(tensor(w_out)), values(tensor(b_out)), tensor(state), false));
 }
 
 // ---------------------------------------------------------------------------------------------- row lookup
@@ -301,7 +304,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 // idx [n, k], weight [n, k] or none -> [n, c]
 Tensor embedding(const Tensor &table, const Optional &weight, const Tensor &idx, double scale, int64_t padding) {
   usable("embedding", {table, tensor(weight), idx});
-  const Tensor t = rows(table), w = tensor(weight);
+  const Tensor t = rows(table), w = values(tensor(weight));
   if (at::GradMode::is_enabled() && (t.requires_grad() || (w.defined() && w.requires_grad()))) return Embedding::apply(t, maybe(w), idx, scale, padding);
   return embedding_raw(t, w, idx, scale);
 }

@@ -957,3 +957,38 @@ def run_camera_sampling_types(device):
             i64 = img.detach().cpu().double().requires_grad_()
             ref, mag = (torch.autograd.grad(point_heads._sample_image_rows(i64, cuv.cpu().to(P), bidx.cpu()), [i64], [d])[0] for d in (dy.cpu().double(), dy.cpu().double().abs()))
             check(g, ref, mag, what="d maps", k=(points + 16) * 2.0 ** -24)
+
+
+def run_negated_views(device):
+    """tensors whose memory holds the other sign (the imaginary part of a conjugate), contiguous and not, in every place of every operator, gradients among them"""
+    from lidarseg3d_amd import blocks
+    gen = torch.Generator().manual_seed(71)
+    z = torch.complex(torch.randn(6, 1, generator=gen), torch.randn(6, 1, generator=gen)).to(device)
+    for neg in (torch._neg_view(tensor(gen, 4, 8, device=device)), z.conj().imag):
+        assert neg.is_neg()
+        plain = neg.clone()
+        assert not plain.is_neg()
+        n, c = plain.shape
+        st = blocks.DropoutState(1, device=device).tensor
+        ix = torch.tensor([[0, 1, 1]] * n, device=device)
+        o, wide = tensor(gen, n, c, device=device), tensor(gen, 9, c, device=device)
+        weights = lambda t: t.expand(n, 3) if c < 3 else t[:, :3]
+        vec = lambda t: torch._neg_view(t[0].neg()) if t.is_neg() else t[0]
+        calls = [lambda t: blocks.dropout(t, 0.25, st, call=0), lambda t: blocks.dropout(t, 0.25, st, call=0, relu=True), lambda t: blocks.residual_norm(t, o, norm=blocks.Norm("layer")),
+                 lambda t: blocks.residual_norm(o, t, norm=blocks.Norm("rms")), lambda t: blocks.residual_norm(o, t, gate=t), lambda t: blocks.residual_norm(o, gate=vec(t)),
+                 lambda t: blocks.residual_norm(o, norm=blocks.Norm("layer", vec(t), vec(t)), norm_in=blocks.Norm("rms", vec(t))), lambda t: blocks.embedding(t, ix),
+                 lambda t: blocks.embedding(wide, ix, weight=weights(t))]
+        for i, f in enumerate(calls):
+            res = []
+            for t in (plain, neg):
+                res.append(f(t))
+                leaf = t.detach()
+                assert leaf.is_neg() == t.is_neg()
+                leaf.requires_grad_()
+                y = f(leaf)
+                dy = torch.ones_like(y)
+                if t.is_neg():
+                    dy = torch._neg_view(-dy)
+                res += [y.detach(), torch.autograd.grad(y, [leaf], [dy])[0]]
+            for a, b in zip(res[:3], res[3:]):
+                assert torch.equal(a, b), i

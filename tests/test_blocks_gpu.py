@@ -273,3 +273,7 @@ def test_one_element_with_a_gate():
 
 def test_camera_sampling_types():
     bc.run_camera_sampling_types(DEV)
+
+
+def test_negated_views():
+    bc.run_negated_views(DEV)

@@ -293,3 +293,7 @@ def test_learned_numbers_are_refused():
 
 def test_camera_sampling_types():
     bc.run_camera_sampling_types("cpu")
+
+
+def test_negated_views():
+    bc.run_negated_views("cpu")
