@@ -612,3 +612,18 @@ def test_single_wave_kernels_keep_their_registers_and_their_blocks():
     f32 = [sum("v_mfma_f32_32x32x2" in ln and "bf16" not in ln for ln in b.splitlines()) for b in blocks]
     assert sum(f32) > 0 and max(f32) == sum(f32), f32  # L = 34: 4 heads x (24 S + 16 + 2 PV) products, all in one block
     assert max(f32) == 4 * (24 + 16 + 2), f32
+
+
+def test_build_entry_compiles_what_is_already_built(monkeypatch):
+    """build() is the check that the sources compile: it asks for a full build whatever stands in the tree"""
+    import __graft_entry__ as entry
+    from lidarseg3d_amd import build as hipbuild
+
+    class Asked(Exception):
+        pass
+
+    def ask(force=False, verbose=False):
+        raise Asked(force)
+    monkeypatch.setattr(hipbuild, "build", ask)
+    with pytest.raises(Asked, match="True"):
+        entry.build()
