@@ -992,3 +992,92 @@ def run_negated_views(device):
                 res += [y.detach(), torch.autograd.grad(y, [leaf], [dy])[0]]
             for a, b in zip(res[:3], res[3:]):
                 assert torch.equal(a, b), i
+
+
+# rows, c, type, index shape, weights, scale, how the tokens fall
+EXACT_LOOKUP = [
+    (1, 8, F32, (30000,), False, 1.0, "one"),          # one row over 3750 tiles of 8: the join looks for its end twice
+    (3, 5, BF16, (52000,), False, 0.5, "few"),         # three rows of about 2170 tiles each
+    (40, 3, F16, (9000, 2), True, 2.0, "empty"),       # two thirds of the entries name no row
+    (9000, 9, F32, (20000,), False, 1.0, "text"),
+    (70, 17, F32, (4097,), False, 1.0, "runs"),
+    (11, 70, BF16, (1500, 3), True, 1.0, "few"),
+]
+# tiles of 16, 32 and 64 entries, more than 2^20 entries (eight to a thread in the sort), many long rows side by side, the camera maps' size
+EXACT_LOOKUP_LARGE = [
+    (700, 64, F32, (300000,), False, 1.0, "text"),
+    (2, 64, BF16, (300007,), False, 0.5, "few"),
+    (50, 128, F32, (300000,), False, 1.0, "uniform"),
+    (5000, 130, F16, (100003, 3), True, 2.0, "empty"),
+    (3, 64, F32, (1200000,), False, 1.0, "few"),
+    (1, 64, F32, (1300001,), False, 1.0, "one"),
+    (100000, 16, F16, (1100000,), False, 1.0, "uniform"),
+    (32, 64, F32, (360000,), False, 1.0, "uniform"),
+    (460800, 48, F32, (360000, 8), True, 1.0, "empty"),
+    (32000, 1024, BF16, (16384,), False, 1.0, "text"),
+    (3000000, 8, F32, (1500000,), False, 1.0, "text"),
+]
+
+
+def exact_indices(gen, rows, shape, how):
+    n = int(np.prod(shape))
+    if how == "one":
+        ix = torch.full((n,), rows - 1)
+    elif how == "text":  # frequency falling with rank: a few rows over many tiles, most over none
+        ix = (rows ** torch.rand(n, generator=gen, dtype=torch.float64) - 1).long().clamp_(0, rows - 1)
+    elif how == "runs":
+        ix = torch.repeat_interleave(torch.arange(rows), torch.arange(rows) * 7 % 90 + 1)[:n]
+        ix = torch.cat([ix, torch.zeros(n - ix.numel(), dtype=torch.int64)])[torch.randperm(n, generator=gen)]
+    else:
+        ix = torch.randint(0, min(rows, 3) if how == "few" else rows, (n,), generator=gen)
+    if how == "empty":
+        ix = torch.where(torch.rand(n, generator=gen) < 0.67, torch.randint(-2, 0, (n,), generator=gen), ix)
+    return ix.reshape(shape)
+
+
+def run_exact_lookup(case, device, seed=0, index=torch.int64):
+    """whole numbers throughout: every product and sum is below 2^24 and exact in 32 bits in any order, so output and gradients equal those of integer arithmetic, rounded
+    to their type once"""
+    from lidarseg3d_amd import blocks
+    rows, c, T, shape, weights, scale, how = case
+    gen = torch.Generator().manual_seed(seed + rows + c)
+    whole = lambda *s: torch.randint(-4, 5, s, generator=gen).to(device)
+    ix = exact_indices(gen, rows, shape, how).to(device)
+    n, k = ix.shape[0], ix.shape[1] if ix.dim() == 2 else 1
+    table, dy = whole(rows, c), whole(n, c)
+    wt = torch.randint(0, 3, shape, generator=gen).to(device) if weights else None
+    padding = rows // 2 if rows > 20 else None
+    t = table.to(T).requires_grad_()
+    w = wt.float().requires_grad_() if weights else None
+    y = blocks.embedding(t, ix.to(index), weight=w, scale=scale, padding_idx=padding)
+    grads = torch.autograd.grad(y, [t] + ([w] if weights else []), [dy.to(T)])
+    flat = ix.reshape(n, k)
+    f = wt.reshape(n, k) if weights else torch.ones_like(flat)
+    out, dt, dw = torch.zeros(n, c, dtype=torch.int64, device=device), torch.zeros(rows, c, dtype=torch.int64, device=device), torch.zeros_like(flat)
+    mag = torch.zeros_like(dt)
+    for j in range(k):
+        at = torch.nonzero(flat[:, j] >= 0)[:, 0]
+        row = table[flat[at, j]]
+        out[at] += f[at, j].unsqueeze(1) * row
+        dw[at, j] = (row * dy[at]).sum(1)
+        if padding is not None:
+            at = at[flat[at, j] != padding]
+        term = f[at, j].unsqueeze(1) * dy[at]
+        dt.index_add_(0, flat[at, j], term)
+        mag.index_add_(0, flat[at, j], term.abs())
+    assert int(mag.max()) < 2 ** 24, "the case is not exact"
+    once = lambda v, type_: (v.double() * scale).to(torch.float32).to(type_)
+    assert torch.equal(y.detach(), once(out, T)), case
+    assert torch.equal(grads[0], once(dt, T)), (case, torch.nonzero(grads[0] != once(dt, T))[:4].tolist())
+    if weights:
+        assert torch.equal(grads[1], once(dw, F32).reshape(grads[1].shape)), case
+
+
+def random_exact_lookup(rng, budget):
+    """a case of at most `budget` values to add, its lengths spread over their logarithm"""
+    log = lambda lo, hi: int(round(np.exp(rng.uniform(np.log(lo), np.log(max(lo, hi))))))
+    c = log(1, 600)
+    k = rng.choice([1, 1, 2, 5])
+    n = log(1, max(1, min(1500000, budget // (c * k))))
+    return (log(1, max(1, min(2000000, 4 * budget // c))), c, rng.choice([F32, BF16, F16]), (n,) if k == 1 else (n, k), k > 1, rng.choice([1.0, 0.5, 2.0]),
+            rng.choice(["empty", "text", "few", "uniform"]) if n * k * 8 < 2 ** 24 else "empty")

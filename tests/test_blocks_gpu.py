@@ -277,3 +277,16 @@ def test_camera_sampling_types():
 
 def test_negated_views():
     bc.run_negated_views(DEV)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
+@pytest.mark.parametrize("case", bc.EXACT_LOOKUP + bc.EXACT_LOOKUP_LARGE, ids=str)
+def test_exact_lookup(case, index):
+    bc.run_exact_lookup(case, DEV, index=index)
+
+
+def test_exact_lookup_of_random_sizes():
+    import random
+    rng = random.Random(6)
+    for i in range(60):
+        bc.run_exact_lookup(bc.random_exact_lookup(rng, 20000000), DEV, seed=i, index=rng.choice([torch.int32, torch.int64]))

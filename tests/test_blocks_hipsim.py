@@ -297,3 +297,15 @@ def test_camera_sampling_types():
 
 def test_negated_views():
     bc.run_negated_views("cpu")
+
+
+@pytest.mark.parametrize("case", bc.EXACT_LOOKUP + [(700, 64, bc.F32, (300000,), False, 1.0, "text")], ids=str)
+def test_exact_lookup(case):
+    bc.run_exact_lookup(case, "cpu")
+
+
+def test_exact_lookup_of_random_sizes():
+    import random
+    rng = random.Random(5)
+    for i in range(60):
+        bc.run_exact_lookup(bc.random_exact_lookup(rng, 60000), "cpu", seed=i, index=rng.choice([torch.int32, torch.int64]))
