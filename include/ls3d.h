@@ -803,7 +803,7 @@ int ls3d_dropout_backward(const void *dy, long long dy_ld, const uint8_t *bits, 
  *   t = in(x);  s = alpha * residual + gate * dropout(t);  y = out(s)
  * residual NULL: s = gate * dropout(t); weight NULL reads as 1, bias NULL as 0; gate: one value per channel [c] or per element [n, c] (of x's type).
  * dtype: x, y, a full gate and their gradients; stream_dtype: residual, s and their gradients - the same type or LS3D_DTYPE_F32.  c <= 8192.
- *   forward : y (out.kind != NONE) and / or s (either may be NULL, not both), stats[n][4] = mean, 1/std of in, mean, 1/std of out (NULL: not wanted)
+ *   forward : y where out.kind != NONE (needed there), s (may be NULL then, needed without a norm), stats[n][4] = mean, 1/std of in, mean, 1/std of out (NULL: not wanted)
  *   backward: from dy and / or ds (NULL: zero) and the forward's inputs and stats: dx, dresidual, dgate ([c] or [n, c]), dw / db of the norms; a NULL
  *             output is not formed.  workspace: ls3d_residual_norm_workspace_bytes(n, c) bytes, 16-byte aligned (needed for dw, db and a channel gate). */
 #define LS3D_NORM_NONE 0

@@ -8,7 +8,8 @@
     loss.backward(); rng.advance()
 
 All three take float32, bfloat16 and float16 tensors with any leading dimensions, run on the current stream of the tensors' device, allocate their
-outputs with torch and give the same bits for the same inputs.  Sums, statistics and parameter gradients are formed in 32 bits and rounded once.
+outputs with torch and give the same bits for the same inputs.  Sums, statistics and parameter gradients are formed in 32 bits and rounded once.  They are
+differentiable once, in reverse mode; tracers, fake tensors, torch.func's transforms and forward-mode tangents are refused.
 
 `use_in_training(model, rng)` puts the training forward of this package's models on them (counter-based dropout, residual and norm in one pass,
 camera sampling with a deterministic gradient)."""
