@@ -1081,3 +1081,18 @@ def random_exact_lookup(rng, budget):
     n = log(1, max(1, min(1500000, budget // (c * k))))
     return (log(1, max(1, min(2000000, 4 * budget // c))), c, rng.choice([F32, BF16, F16]), (n,) if k == 1 else (n, k), k > 1, rng.choice([1.0, 0.5, 2.0]),
             rng.choice(["empty", "text", "few", "uniform"]) if n * k * 8 < 2 ** 24 else "empty")
+
+
+def run_inputs_changed_before_the_backward_pass(device):
+    """x, residual or gate changed in place after the forward pass: refused, whatever the number of dimensions the rows were made of"""
+    import pytest
+
+    from lidarseg3d_amd import blocks
+    for shape in ((8,), (3, 8), (2, 3, 8)):
+        for which in ("x", "residual", "gate"):
+            w = torch.ones(8, device=device, requires_grad=True)
+            t = {k: torch.ones(shape, device=device) for k in ("x", "residual", "gate")}
+            y = blocks.residual_norm(t["x"], t["residual"], gate=t["gate"], norm=blocks.Norm("rms", w))
+            t[which].add_(1)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()

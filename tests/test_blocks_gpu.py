@@ -290,3 +290,7 @@ def test_exact_lookup_of_random_sizes():
     rng = random.Random(6)
     for i in range(60):
         bc.run_exact_lookup(bc.random_exact_lookup(rng, 20000000), DEV, seed=i, index=rng.choice([torch.int32, torch.int64]))
+
+
+def test_inputs_changed_before_the_backward_pass():
+    bc.run_inputs_changed_before_the_backward_pass(DEV)
